@@ -23,9 +23,13 @@ BUILD = os.path.join(ROOT, 'build', 'hip')
 ARCH = os.environ.get('KFAC_HIP_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 # kernarg preload: the first kernel arguments arrive in SGPRs, so a latency-
-# bound launch does not start with a scalar load round trip
+# bound launch does not start with a scalar load round trip.
+# packed FP32 instructions off: the compiler forms them from ordinary float
+# code, and some of their forms have given wrong results on this hardware now
+# and then (the host pass does not know the feature and says so: harmless)
 FLAGS = ['-O3', '-std=c++17', '-fPIC', '--offload-arch=' + ARCH, '-munsafe-fp-atomics',
-         '-Wno-unused-result', '-mllvm', '-amdgpu-kernarg-preload-count=16']
+         '-Wno-unused-result', '-mllvm', '-amdgpu-kernarg-preload-count=16',
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
 
 # no vendor math library: every kernel is hand-written (the HIP runtime only)

@@ -5,13 +5,16 @@ example (the reference itself only ships an LSTM LM).  Every projection is an
 nn.Linear on (B, T, D) activations, so each K-FAC Linear factor folds B*T into
 the SYRK row dimension (layers/linear.py); attention uses
 F.scaled_dot_product_attention.  K-FAC skips the embedding
-(`skip_layers=['embedding']`); LayerNorm is not a K-FAC module.
+(`skip_layers=['embedding']`); LayerNorm is not a K-FAC module: it runs on the
+framework's own kernels, the residual add in front of ln2 with it (ops/ln.py).
 """
 import math
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..modules import LayerNorm
 
 __all__ = ['TransformerLM', 'Block']
 
@@ -20,10 +23,10 @@ class Block(nn.Module):
     def __init__(self, d_model, n_heads, d_ff, dropout=0.0):
         super().__init__()
         self.n_heads = n_heads
-        self.ln1 = nn.LayerNorm(d_model)
+        self.ln1 = LayerNorm(d_model)
         self.qkv = nn.Linear(d_model, 3 * d_model)
         self.proj = nn.Linear(d_model, d_model)
-        self.ln2 = nn.LayerNorm(d_model)
+        self.ln2 = LayerNorm(d_model)
         self.fc1 = nn.Linear(d_model, d_ff)
         self.fc2 = nn.Linear(d_ff, d_model)
         self.dropout = dropout
@@ -35,8 +38,8 @@ class Block(nn.Module):
         q, k, v = (t.transpose(1, 2) for t in (q, k, v))
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True,
                                            dropout_p=self.dropout if self.training else 0.0)
-        x = x + self.proj(a.transpose(1, 2).reshape(B, T, D))
-        x = x + self.fc2(F.gelu(self.fc1(self.ln2(x))))
+        h, x = self.ln2(x, self.proj(a.transpose(1, 2).reshape(B, T, D)))   # x = x + proj
+        x = x + self.fc2(F.gelu(self.fc1(h)))
         return x
 
 
@@ -48,7 +51,7 @@ class TransformerLM(nn.Module):
         self.pos = nn.Embedding(max_len, d_model)
         self.blocks = nn.ModuleList([Block(d_model, n_heads, d_ff, dropout)
                                      for _ in range(n_layers)])
-        self.ln_f = nn.LayerNorm(d_model)
+        self.ln_f = LayerNorm(d_model)
         self.head = nn.Linear(d_model, vocab, bias=False)
         for m in self.modules():
             if isinstance(m, nn.Linear):

@@ -5,10 +5,12 @@ factors    implicit-im2col MFMA SYRK + fused EMA (K1-K5)
 eigen      batched Jacobi eigensolver (K6) / Cholesky inverse (K9)
 precond    eigenbasis preconditioning, grouped KL-dot + apply (K7, K8, K10, K11)
 comm_pack  triu pack/unpack for the factor all-reduce arena (K12)
+bn         fused BatchNorm (+ add) (+ ReLU) of the image models
+ln         layer norm (+ residual add) of the Transformer LM
 """
-from . import _lib, factors, eigen, precond, comm_pack
+from . import _lib, factors, eigen, precond, comm_pack, bn, ln
 
-__all__ = ['_lib', 'factors', 'eigen', 'precond', 'comm_pack', 'native_available']
+__all__ = ['_lib', 'factors', 'eigen', 'precond', 'comm_pack', 'bn', 'ln', 'native_available']
 
 
 def native_available():

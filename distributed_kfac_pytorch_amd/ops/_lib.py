@@ -7,11 +7,13 @@ captured into hipGraphs.  On a GPU process the library is REQUIRED: the
 ops fail loudly instead of silently falling back (the CPU plumbing path is
 used only for CPU tensors).
 """
+import contextlib
 import ctypes
 import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_HERE, '_native', 'libkfac_hip.so')
@@ -151,6 +153,11 @@ _SIGS = {
     'kfac_dc_ws_bytes': [c_int],
     'kfac_dc_set_fast_scan': [c_int],
     'kfac_dc_info_offset': [c_int],
+    'kfac_ln_ws_floats': [c_ll, c_ll],
+    'kfac_ln_forward': [c_vp, c_ll, c_int, c_vp, c_ll, c_int, c_vp, c_int, c_vp, c_int, c_vp,
+                        c_int, c_vp, c_vp, c_vp, c_ll, c_ll, c_f, c_vp],
+    'kfac_ln_backward': [c_vp, c_ll, c_int, c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_int,
+                         c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_ll, c_ll, c_vp],
     'kfac_bn_ws_floats': [c_ll, c_int],
     'kfac_bn_forward': [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_ll,
                         c_int, ctypes.c_float, ctypes.c_float, c_int, c_vp],
@@ -163,7 +170,7 @@ _RESTYPES = {'kfac_dc_ws_bytes': c_ll, 'kfac_sy2sb_ws_floats': c_ll,
              'kfac_reduce_ws_floats': c_ll, 'kfac_syrk_splits': c_ll,
              'kfac_chol_ws_bytes': c_ll, 'kfac_chol_info_offset': c_ll,
              'kfac_syrk_problem_set_part': None, 'kfac_syrk_problem_set_dscale': None,
-             'kfac_bn_ws_floats': c_ll, 'kfac_event_create': c_vp}
+             'kfac_bn_ws_floats': c_ll, 'kfac_ln_ws_floats': c_ll, 'kfac_event_create': c_vp}
 
 
 def _load():
@@ -219,6 +226,28 @@ def use_native(t):
         return False
     lib()  # loud failure on a GPU tensor without the library
     return True
+
+
+_no_guard = contextlib.nullcontext()
+
+
+def device_guard(device):
+    """Context in which `device` is the current one: a launch goes to the current
+    device, also where its tensors and stream belong to another."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _no_guard
+    return torch.cuda.device(device)
+
+
+def plain_tensors(*tensors):
+    """True where raw pointers may be taken: ordinary tensors, and neither a
+    functorch transform, a forward-mode level nor a compile trace around them
+    (each of these needs torch operations that it knows)."""
+    if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active() \
+            or forward_ad._current_level >= 0:
+        return False
+    return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter
+               for t in tensors)
 
 
 def stream(device=None):

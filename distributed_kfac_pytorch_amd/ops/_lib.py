@@ -158,6 +158,15 @@ _SIGS = {
                         c_int, c_vp, c_vp, c_vp, c_ll, c_ll, c_f, c_vp],
     'kfac_ln_backward': [c_vp, c_ll, c_int, c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_int,
                          c_vp, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_vp, c_ll, c_ll, c_vp],
+    'kfac_vocab_top_max': [],
+    'kfac_logprob_forward': [c_vp, c_ll, c_int, c_ll, c_ll, c_f, c_vp, c_ll, c_int, c_vp, c_vp,
+                             c_vp, c_vp, c_vp, c_vp],
+    'kfac_logprob_backward': [c_vp, c_ll, c_int, c_ll, c_ll, c_f, c_vp, c_ll, c_vp, c_vp, c_vp,
+                              c_ll, c_vp, c_ll, c_vp, c_vp],
+    'kfac_distill_forward': [c_vp, c_ll, c_int, c_ll, c_ll, c_f, c_vp, c_vp, c_int, c_int, c_vp,
+                             c_vp, c_vp],
+    'kfac_distill_backward': [c_vp, c_ll, c_int, c_ll, c_ll, c_f, c_vp, c_vp, c_int, c_int, c_vp,
+                              c_vp, c_ll, c_vp, c_vp],
     'kfac_bn_ws_floats': [c_ll, c_int],
     'kfac_bn_forward': [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_ll,
                         c_int, ctypes.c_float, ctypes.c_float, c_int, c_vp],

@@ -14,7 +14,10 @@ this is a working rewrite of its behaviour:
     reference) and, with --tied, the decoder too (the reference's
     --register-tied path fed integer token ids into a Linear factor and
     cannot work; the tied weight gets plain SGD gradients);
-  * HYBRID_OPT with grad_worker_fraction 0.25 is the BASELINE LM config.
+  * HYBRID_OPT with grad_worker_fraction 0.25 is the BASELINE LM config;
+  * --save writes the trained weights; --teacher takes such a file (a model of
+    the same kind, its sizes by --teacher-emsize / --teacher-nlayers) and trains
+    the student on the teacher's --distill-topk likeliest tokens as well.
 
 Launch: python -m torch.distributed.run --nproc-per-node 8 --master-addr
 127.0.0.1 examples/torch_language_model.py --model transformer ...
@@ -33,6 +36,8 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import distributed_kfac_pytorch_amd as kfac  # noqa: E402
 from distributed_kfac_pytorch_amd.models import LSTMModel, TransformerLM  # noqa: E402
+from distributed_kfac_pytorch_amd.ops.vocab import (token_logprobs,  # noqa: E402
+                                                    topk_distill_loss)
 from distributed_kfac_pytorch_amd.parallel import launch  # noqa: E402
 from examples.rnn_utils.utils import Corpus, batchify, bptt_batches  # noqa: E402
 from examples.utils import Metric  # noqa: E402
@@ -77,6 +82,15 @@ def parse(argv=None):
     p.add_argument('--precond-precision', default='bf16x6', choices=['bf16x6', 'fp32', 'bf16x3'],
                    help='preconditioning GEMMs: bf16x6 = six bf16 MFMA products per fp32 '
                         'product (fp32-level error), fp32 = exact f32 MFMA, bf16x3 = ~1e-5')
+    p.add_argument('--save', default=None, help='write the trained weights to this file')
+    p.add_argument('--teacher', default=None, help='weights (--save) of a teacher to distill from')
+    p.add_argument('--teacher-emsize', type=int, default=None, help='default: --emsize')
+    p.add_argument('--teacher-nhid', type=int, default=None, help='default: --nhid')
+    p.add_argument('--teacher-nlayers', type=int, default=None, help='default: --nlayers')
+    p.add_argument('--distill-topk', type=int, default=16)
+    p.add_argument('--distill-temperature', type=float, default=2.0)
+    p.add_argument('--distill-weight', type=float, default=0.5,
+                   help='share of the distillation term in the loss')
     p.add_argument('--verbose', action='store_true')
     return p.parse_args(argv)
 
@@ -84,6 +98,28 @@ def parse(argv=None):
 def get_batch(source, i, bptt):
     seq_len = min(bptt, len(source) - 1 - i)
     return source[i:i + seq_len], source[i + 1:i + 1 + seq_len].reshape(-1)
+
+
+def build_model(args, ntokens, emsize, nhid, nlayers):
+    if args.model == 'lstm':
+        return LSTMModel(ntokens, emsize, nhid, nlayers, args.dropout, args.tied)
+    return TransformerLM(ntokens, d_model=emsize, n_layers=nlayers, n_heads=args.nheads,
+                         d_ff=4 * emsize, max_len=max(args.bptt, 64), dropout=0.0)
+
+
+def load_teacher(args, ntokens, device):
+    teacher = build_model(args, ntokens, args.teacher_emsize or args.emsize,
+                          args.teacher_nhid or args.nhid, args.teacher_nlayers or args.nlayers)
+    teacher.load_state_dict(torch.load(args.teacher, map_location='cpu', weights_only=True))
+    return teacher.to(device).eval().requires_grad_(False)
+
+
+def distill_loss(args, out, teacher_out):
+    """T^2 times the mean divergence from the teacher's likeliest tokens: T^2 keeps
+    the gradient's size over temperatures."""
+    top = token_logprobs(teacher_out, top_k=min(args.distill_topk, teacher_out.size(-1)))
+    T = args.distill_temperature
+    return T * T * topk_distill_loss(out, top.top_ids, top.top_logprobs, T).mean()
 
 
 def run_model(model, data, hidden, args):
@@ -108,13 +144,7 @@ def main(argv=None):
     val = batchify(corpus.valid, args.eval_batch_size)
     train, val = train.to(device), val.to(device)
 
-    if args.model == 'lstm':
-        model = LSTMModel(corpus.ntokens, args.emsize, args.nhid, args.nlayers, args.dropout,
-                          args.tied)
-    else:
-        model = TransformerLM(corpus.ntokens, d_model=args.emsize, n_layers=args.nlayers,
-                              n_heads=args.nheads, d_ff=4 * args.emsize,
-                              max_len=max(args.bptt, 64), dropout=0.0)
+    model = build_model(args, corpus.ntokens, args.emsize, args.nhid, args.nlayers)
     model = model.to(device)
     ddp = launch.wrap_ddp(model, device)
 
@@ -135,17 +165,24 @@ def main(argv=None):
                         verbose=args.verbose and rank == 0)
     sched = torch.optim.lr_scheduler.StepLR(optimizer, args.lr_decay_epoch, args.lr_decay_rate)
     criterion = nn.CrossEntropyLoss()
+    teacher = load_teacher(args, corpus.ntokens, device) if args.teacher else None
     history = []
     for epoch in range(args.epochs):
         model.train()
         t0 = time.time()
         hidden = model.init_hidden(train.size(1)) if args.model == 'lstm' else None
+        t_hidden = None if hidden is None or teacher is None else \
+            teacher.init_hidden(train.size(1))
         loss_m = Metric('train_loss')
         for i in bptt_batches(train, args.bptt):
             data, targets = get_batch(train, i, args.bptt)
             optimizer.zero_grad()
             out, hidden = run_model(ddp, data, hidden, args)
             loss = criterion(out.reshape(-1, out.size(-1)), targets)
+            if teacher is not None:
+                with torch.no_grad():
+                    t_out, t_hidden = run_model(teacher, data, t_hidden, args)
+                loss = torch.lerp(loss, distill_loss(args, out, t_out), args.distill_weight)
             loss.backward()
             torch.nn.utils.clip_grad_norm_(model.parameters(), args.clip)
             if pre is not None:
@@ -153,20 +190,27 @@ def main(argv=None):
             optimizer.step()
             loss_m.update(loss)
         model.eval()
-        val_m = Metric('val_loss')
+        val_m, ent_m, top_m = Metric('val_loss'), Metric('val_entropy'), Metric('val_top1')
         with torch.no_grad():
             hidden = model.init_hidden(val.size(1)) if args.model == 'lstm' else None
             for i in bptt_batches(val, args.bptt):
                 data, targets = get_batch(val, i, args.bptt)
                 out, hidden = run_model(model, data, hidden, args)
                 val_m.update(criterion(out.reshape(-1, out.size(-1)), targets))
+                r = token_logprobs(out, top_k=1, entropy=True)
+                ent_m.update(r.entropy.mean())
+                top_m.update((r.top_ids.reshape(-1) == targets).float().mean())
         sched.step()
         tl, vl = float(loss_m.avg), float(val_m.avg)
         rec = {'epoch': epoch + 1, 'train_loss': tl, 'train_ppl': math.exp(min(tl, 50)),
-               'val_loss': vl, 'val_ppl': math.exp(min(vl, 50)), 'time': time.time() - t0}
+               'val_loss': vl, 'val_ppl': math.exp(min(vl, 50)),
+               'val_entropy': float(ent_m.avg), 'val_top1': float(top_m.avg),
+               'time': time.time() - t0}
         history.append(rec)
         if rank == 0:
             print(json.dumps(rec), flush=True)
+    if args.save and rank == 0:
+        torch.save(model.state_dict(), args.save)
     return history
 
 

@@ -12,7 +12,7 @@
 // sum are held in fp32, the variance about the mean (two passes over the row).
 // The sums over rows (dw, db) run over fixed row chunks and then over the
 // chunks in order: no atomics, bitwise reproducible.
-#include "common.h"
+#include "rows.h"
 
 namespace {
 
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const Fwd a) {
     if (a.b) v += ld_any(a.b, i, a.bdt);
     st_any(a.y, yo + i, a.ydt, v);
   }
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && a.mean) {
     a.mean[row] = mu;
     a.rstd[row] = rstd;
   }
@@ -133,47 +133,370 @@ __global__ __launch_bounds__(NT) void ln_param_part_kernel(const Bwd a) {
   a.part[(2LL * blockIdx.y + 1) * a.D + c] = db;
 }
 
-__global__ __launch_bounds__(NT) void ln_param_sum_kernel(const Bwd a) {
-  const long long c = (long long)blockIdx.x * NT + threadIdx.x;
-  if (c >= a.D) return;
-  float dw = 0.f, db = 0.f;
-  for (int k = 0; k < a.chunks; ++k) {
-    dw += a.part[2LL * k * a.D + c];
-    db += a.part[(2LL * k + 1) * a.D + c];
+// ---------------------------------------------------------------------------
+// Rows of V .. 16384 elements: a row is held in the registers of TR threads, E
+// elements each in 16-byte accesses, so that x, z (forward) and dy, s, ds
+// (backward) are read once and the statistics are taken from registers.
+// Workgroups of 256 threads hold 256 / TR rows at a time (TR >= 256: one) and
+// stride over the rows.
+
+template <int TR> struct RowSum {      // sums over the TR threads of a row
+  static constexpr int W = TR / 64;    // waves a row
+  static constexpr int BT = TR < 256 ? 256 : TR;
+  // red: one float a wave of the workgroup, not read or written between this
+  // call's barrier and the next call's (two buffers in turn)
+  static __device__ __forceinline__ float sum(float v, float* red) {
+    v += dpp_f<0xB1>(v);               // quad_perm [1,0,3,2]
+    v += dpp_f<0x4E>(v);               // quad_perm [2,3,0,1]
+    v += dpp_f<0x141>(v);              // row_half_mirror
+    v += dpp_f<0x140>(v);              // row_mirror: 16 lanes
+    if (TR >= 32) v = swap_sum16(v);
+    if (TR >= 64) v = swap_sum32(v);
+    if (TR <= 64) return v;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    kfac_lds_barrier();
+    const int w0 = wave / (W ? W : 1) * W;
+    float r = red[w0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) r += red[w0 + i];
+    return r;
   }
-  if (a.dw) st_any(a.dw, c, a.wdt, dw);
-  if (a.db) st_any(a.db, c, a.bdt, db);
+};
+
+// z's or dy's E elements in another type than the stream's (uniform over the launch)
+template <int V, int R>
+__device__ __forceinline__ void load_other(const void* p, long long off, int dt, int t0, int step,
+                                           int n, float* f) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int i = t0 + r * step + e;
+      f[r * V + e] = i < n ? ld_any(p, off + i, dt) : 0.f;
+    }
+}
+template <int V, int R>
+__device__ __forceinline__ void store_other(void* p, long long off, int dt, int t0, int step,
+                                            int n, const float* f) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int i = t0 + r * step + e;
+      if (i < n) st_any(p, off + i, dt, f[r * V + e]);
+    }
 }
 
-int param_chunks(long long rows) {
-  const long long c = (rows + 63) / 64;
-  return (int)(c < 512 ? c : 512);
+template <int DT, int TR, int E, bool TAIL>
+__global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>(), R = E / V, BT = RowSum<TR>::BT, RPW = BT / TR;
+  __shared__ float red[2][BT / 64];
+  const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
+  const int D = (int)a.D, t0 = t * V, step = TR * V;
+  const float inv_d = 1.f / (float)D;
+  float w[E], b[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) { w[e] = 1.f; b[e] = 0.f; }
+  if (a.w) load_other<V, R>(a.w, 0, a.wdt, t0, step, D, w);
+  if (a.b) load_other<V, R>(a.b, 0, a.bdt, t0, step, D, b);
+  for (long long base = (long long)blockIdx.x * RPW; base < a.rows;
+       base += (long long)gridDim.x * RPW) {
+    const bool live = base + sub < a.rows;
+    const long long row = live ? base + sub : a.rows - 1;
+    const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
+    float f[E];
+    u32x4n raw[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) raw[r] = load_vec<DT, TAIL>(x, t0 + r * step, D);
+    if (a.z) {
+      float g[E];
+      if (a.zdt == DT) {
+        const AS1 raw_t* z = gptr((const raw_t*)a.z) + row * a.ldz;
+        u32x4n zraw[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) zraw[r] = load_vec<DT, TAIL>(z, t0 + r * step, D);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          vec_to_f32<DT>(clip_vec<DT, TAIL>(zraw[r], t0 + r * step, D), g + r * V);
+      } else {
+        load_other<V, R>(a.z, row * a.ldz, a.zdt, t0, step, D, g);
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int i = t0 + r * step;
+        vec_to_f32<DT>(clip_vec<DT, TAIL>(raw[r], i, D), f + r * V);
+#pragma unroll
+        for (int e = 0; e < V; ++e)       // the sum as it is stored is what is normed
+          f[r * V + e] = DTypeTraits<DT>::to_f32(
+              DTypeTraits<DT>::from_f32(f[r * V + e] + g[r * V + e]));
+        if (live) store_vec<DT, TAIL>(gptr((raw_t*)a.s) + row * D, i, D, f + r * V);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        vec_to_f32<DT>(clip_vec<DT, TAIL>(raw[r], t0 + r * step, D), f + r * V);
+    }
+    float acc = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc += f[e];
+    const float mu = RowSum<TR>::sum(acc, red[0]) * inv_d;
+    acc = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = f[r * V + e] - mu;
+        f[r * V + e] = d;
+        acc = fmaf(d, t0 + r * step + e < D ? d : 0.f, acc);
+      }
+    const float rstd = 1.f / sqrtf(RowSum<TR>::sum(acc, red[1]) * inv_d + a.eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = fmaf(f[e] * rstd, w[e], b[e]);
+    if (live) {
+      if (a.ydt == DT) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          store_vec<DT, TAIL>(gptr((raw_t*)a.y) + row * D, t0 + r * step, D, f + r * V);
+      } else {
+        store_other<V, R>(a.y, row * D, a.ydt, t0, step, D, f);
+      }
+      if (t == 0 && a.mean) {
+        a.mean[row] = mu;
+        a.rstd[row] = rstd;
+      }
+    }
+  }
+}
+
+// dx (and dz), and the workgroup's rows' part of dw and db in registers: two
+// floats an element, added over the workgroup's row groups at the end
+template <int DT, int TR, int E, bool TAIL>
+__global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>(), R = E / V, BT = RowSum<TR>::BT, RPW = BT / TR;
+  __shared__ float red[2][BT / 64];
+  __shared__ float fold[RPW > 1 ? RPW * TR * E : 1];
+  const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
+  const int D = (int)a.D, t0 = t * V, step = TR * V;
+  const float inv_d = 1.f / (float)D;
+  float w[E], dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) { w[e] = 1.f; dw[e] = 0.f; db[e] = 0.f; }
+  if (a.w) load_other<V, R>(a.w, 0, a.wdt, t0, step, D, w);
+  for (long long base = (long long)blockIdx.x * RPW; base < a.rows;
+       base += (long long)gridDim.x * RPW) {
+    const bool live = base + sub < a.rows;
+    const long long row = live ? base + sub : a.rows - 1;
+    const AS1 raw_t* s = gptr((const raw_t*)a.s) + row * a.lds;
+    const AS1 raw_t* ds = gptr((const raw_t*)a.ds) + row * a.ldds;
+    float h[E], g[E];
+    u32x4n sraw[R], eraw[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) sraw[r] = load_vec<DT, TAIL>(s, t0 + r * step, D);
+    if (a.ds) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) eraw[r] = load_vec<DT, TAIL>(ds, t0 + r * step, D);
+    }
+    if (a.ydt == DT) {
+      const AS1 raw_t* dy = gptr((const raw_t*)a.dy) + row * a.lddy;
+      u32x4n graw[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) graw[r] = load_vec<DT, TAIL>(dy, t0 + r * step, D);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        vec_to_f32<DT>(clip_vec<DT, TAIL>(graw[r], t0 + r * step, D), g + r * V);
+    } else {
+      load_other<V, R>(a.dy, row * a.lddy, a.ydt, t0, step, D, g);
+    }
+    const float mu = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      vec_to_f32<DT>(clip_vec<DT, TAIL>(sraw[r], t0 + r * step, D), h + r * V);
+    float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      h[e] = (h[e] - mu) * rstd;
+      if (!live) g[e] = 0.f;
+      dw[e] = fmaf(g[e], h[e], dw[e]);           // past the row's end g is 0
+      db[e] += g[e];
+      g[e] *= w[e];
+      c1 += g[e];
+      c2 = fmaf(g[e], h[e], c2);
+    }
+    if (a.dx) {
+      c1 = RowSum<TR>::sum(c1, red[0]) * inv_d;
+      c2 = RowSum<TR>::sum(c2, red[1]) * inv_d;
+#pragma unroll
+      for (int e = 0; e < E; ++e) g[e] = rstd * (g[e] - c1 - h[e] * c2);
+      if (a.ds) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          vec_to_f32<DT>(clip_vec<DT, TAIL>(eraw[r], t0 + r * step, D), h + r * V);
+#pragma unroll
+          for (int e = 0; e < V; ++e) g[r * V + e] += h[r * V + e];
+        }
+      }
+      if (live) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          store_vec<DT, TAIL>(gptr((raw_t*)a.dx) + row * D, t0 + r * step, D, g + r * V);
+        if (a.dz) store_other<V, R>(a.dz, row * D, a.zdt, t0, step, D, g);
+      }
+    }
+  }
+  if (!a.part) return;
+  float* out = a.part + 2LL * blockIdx.x * D;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float* v = k ? db : dw;
+    if (RPW > 1) {                        // row groups added in order
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) fold[(sub * E + e) * TR + t] = v[e];
+      __syncthreads();
+      if (sub == 0) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          for (int j = 1; j < RPW; ++j) v[e] += fold[(j * E + e) * TR + t];
+      }
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        store_vec<KDT_F32, true>(gptr(out + (long long)k * D), t0 + r * step, D, v + r * V);
+      if (V == 8) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+          store_vec<KDT_F32, true>(gptr(out + (long long)k * D), t0 + r * step + 4, D,
+                                   v + r * V + 4);
+      }
+    }
+  }
+}
+
+// dw, db from the parts, 32 columns a workgroup: each of 32 threads a column
+// adds every 32nd part in order, then the 32 sums are added in order
+__global__ __launch_bounds__(1024) void ln_param_sum_kernel(const Bwd a) {
+  __shared__ float sh[2][32][33];
+  const int cx = threadIdx.x & 31, k0 = threadIdx.x >> 5;
+  const long long c = (long long)blockIdx.x * 32 + cx;
+  float dw = 0.f, db = 0.f;
+  if (c < a.D) {
+#pragma unroll 4
+    for (int k = k0; k < a.chunks; k += 32) {
+      dw += a.part[2LL * k * a.D + c];
+      db += a.part[(2LL * k + 1) * a.D + c];
+    }
+  }
+  sh[0][k0][cx] = dw;
+  sh[1][k0][cx] = db;
+  __syncthreads();
+  if (k0 < 2 && c < a.D) {
+    float v = 0.f;
+    for (int k = 0; k < 32; ++k) v += sh[k0][k][cx];
+    if (k0 == 0 && a.dw) st_any(a.dw, c, a.wdt, v);
+    if (k0 == 1 && a.db) st_any(a.db, c, a.bdt, v);
+  }
 }
 
 bool dtype_ok(int dt) { return dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16; }
 
+// Threads and elements a row (TR, E): the narrowest that hold D.
+constexpr long long LONG_ROW = 16384;     // longer rows: the kernels that loop over the row
+
+#define LN_SIZES(F) F(16, 8) F(32, 8) F(64, 8) F(64, 16) F(128, 16) F(256, 16) F(512, 16) F(1024, 16)
+
+bool looped(int dt, long long D) { return D > LONG_ROW || D < (dt == KDT_F32 ? 4 : 8); }
+
+// threads a row
+int row_threads(long long D) {
+  int n = 0;
+#define F(TR, E) if (!n && D <= TR * E) n = TR;
+  LN_SIZES(F)
+#undef F
+  return n;
+}
+
+// workgroups that stride over the rows: at most `cap` of 256 threads (fewer, wider ones alike)
+long long row_blocks(long long rows, long long D, long long cap) {
+  const int tr = row_threads(D);
+  const long long per = tr < 256 ? 256 / tr : 1, most = tr > 256 ? cap * 256 / tr : cap;
+  const long long n = (rows + per - 1) / per;
+  return n < most ? n : most;
+}
+
+constexpr long long FWD_BLOCKS = 4096, BWD_BLOCKS = 1024;
+
+int param_chunks(int dt, long long rows, long long D) {
+  if (!looped(dt, D)) return (int)row_blocks(rows, D, BWD_BLOCKS);
+  const long long c = (rows + 63) / 64;
+  return (int)(c < 512 ? c : 512);
+}
+
+template <int DT, int TR, int E>
+void launch_fwd(const Fwd& a, hipStream_t st) {
+  const dim3 grid((unsigned)row_blocks(a.rows, a.D, FWD_BLOCKS)), block(RowSum<TR>::BT);
+  if (a.D % row_vec<DT>())
+    hipLaunchKernelGGL((ln_fwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((ln_fwd_kernel<DT, TR, E, false>), grid, block, 0, st, a);
+}
+template <int DT, int TR, int E>
+void launch_bwd(const Bwd& a, hipStream_t st) {
+  const dim3 grid((unsigned)row_blocks(a.rows, a.D, BWD_BLOCKS)), block(RowSum<TR>::BT);
+  if (a.D % row_vec<DT>())
+    hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, false>), grid, block, 0, st, a);
+}
+template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
+  const int n = row_threads(a.D);
+  bool done = false;
+#define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_fwd<DT, TR, E>(a, st); done = true; }
+  LN_SIZES(F)
+#undef F
+}
+template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
+  const int n = row_threads(a.D);
+  bool done = false;
+#define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_bwd<DT, TR, E>(a, st); done = true; }
+  LN_SIZES(F)
+#undef F
+}
+
 }  // namespace
 
 // floats of the workspace of one backward call that asks for dw or db
-KFAC_API long long kfac_ln_ws_floats(long long rows, long long D) {
-  return 2LL * param_chunks(rows) * D;
+KFAC_API long long kfac_ln_ws_floats(int sdt, long long rows, long long D) {
+  return 2LL * param_chunks(sdt, rows, D) * D;
 }
 
-// z and s null: the norm of x.  w, b may be null.  mean, rstd: fp32, one a row.
+// z and s null: the norm of x.  w, b may be null; mean, rstd (fp32, one a row)
+// may be null where no backward pass follows.
 KFAC_API int kfac_ln_forward(const void* x, long long ldx, int sdt, const void* z, long long ldz,
                              int zdt, const void* w, int wdt, const void* b, int bdt, void* y,
                              int ydt, void* s, float* mean, float* rstd, long long rows,
                              long long D, float eps, hipStream_t stream) {
   if (rows <= 0 || rows > 0x7fffffffLL || D <= 0 || !dtype_ok(sdt) || !dtype_ok(ydt) ||
-      (z && (!s || !dtype_ok(zdt))) || (w && !dtype_ok(wdt)) || (b && !dtype_ok(bdt)))
+      (z && (!s || !dtype_ok(zdt))) || (w && !dtype_ok(wdt)) || (b && !dtype_ok(bdt)) ||
+      !mean != !rstd)
     return -2;
   Fwd a = {x, z, w, b, y, s, mean, rstd, ldx, ldz, rows, D, sdt, zdt, wdt, bdt, ydt, eps};
-  hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
+  if (looped(sdt, D))
+    hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
+  else if (sdt == KDT_F32)
+    launch_fwd_any<KDT_F32>(a, stream);
+  else if (sdt == KDT_BF16)
+    launch_fwd_any<KDT_BF16>(a, stream);
+  else
+    launch_fwd_any<KDT_F16>(a, stream);
   return (int)hipGetLastError();
 }
 
 // ds (the gradient that reaches s itself), dx, dz, dw, db may be null; part
-// is read only where dw or db is asked for
+// (kfac_ln_ws_floats) is needed where dw or db is asked for
 KFAC_API int kfac_ln_backward(const void* dy, long long lddy, int ydt, const void* ds,
                               long long ldds, const void* s, long long lds, int sdt,
                               const void* w, int wdt, int bdt, const float* mean,
@@ -183,13 +506,22 @@ KFAC_API int kfac_ln_backward(const void* dy, long long lddy, int ydt, const voi
       (dz && (!dx || !dtype_ok(zdt))) || ((w || dw) && !dtype_ok(wdt)) ||
       (db && !dtype_ok(bdt)) || ((dw || db) && !part))
     return -2;
-  Bwd a = {dy, ds, s, w, mean, rstd, dx, dz, dw, db, part, lddy, ldds, lds, rows, D,
-           sdt, zdt, wdt, bdt, ydt, param_chunks(rows)};
-  if (dx) hipLaunchKernelGGL(ln_bwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
-  if (dw || db) {
-    const unsigned cols = (unsigned)((D + NT - 1) / NT);
-    hipLaunchKernelGGL(ln_param_part_kernel, dim3(cols, a.chunks), dim3(NT), 0, stream, a);
-    hipLaunchKernelGGL(ln_param_sum_kernel, dim3(cols), dim3(NT), 0, stream, a);
+  Bwd a = {dy, ds, s, w, mean, rstd, dx, dz, dw, db, dw || db ? part : nullptr, lddy, ldds, lds,
+           rows, D, sdt, zdt, wdt, bdt, ydt, param_chunks(sdt, rows, D)};
+  if (looped(sdt, D)) {
+    if (dx) hipLaunchKernelGGL(ln_bwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
+    if (a.part)
+      hipLaunchKernelGGL(ln_param_part_kernel, dim3((unsigned)((D + NT - 1) / NT), a.chunks),
+                         dim3(NT), 0, stream, a);
+  } else if (sdt == KDT_F32) {
+    launch_bwd_any<KDT_F32>(a, stream);
+  } else if (sdt == KDT_BF16) {
+    launch_bwd_any<KDT_BF16>(a, stream);
+  } else {
+    launch_bwd_any<KDT_F16>(a, stream);
   }
+  if (a.part)
+    hipLaunchKernelGGL(ln_param_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(1024), 0,
+                       stream, a);
   return (int)hipGetLastError();
 }

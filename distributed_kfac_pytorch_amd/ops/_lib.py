@@ -153,7 +153,7 @@ _SIGS = {
     'kfac_dc_ws_bytes': [c_int],
     'kfac_dc_set_fast_scan': [c_int],
     'kfac_dc_info_offset': [c_int],
-    'kfac_ln_ws_floats': [c_ll, c_ll],
+    'kfac_ln_ws_floats': [c_int, c_ll, c_ll],
     'kfac_ln_forward': [c_vp, c_ll, c_int, c_vp, c_ll, c_int, c_vp, c_int, c_vp, c_int, c_vp,
                         c_int, c_vp, c_vp, c_vp, c_ll, c_ll, c_f, c_vp],
     'kfac_ln_backward': [c_vp, c_ll, c_int, c_vp, c_ll, c_vp, c_ll, c_int, c_vp, c_int, c_int,

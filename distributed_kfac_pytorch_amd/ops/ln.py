@@ -139,7 +139,7 @@ def _backward(ctx, s, weight, bias, stats, dy, ds):
     dl = None if same else torch.empty(s.shape, dtype=low, device=s.device)
     dw = torch.empty(weight.shape, dtype=weight.dtype, device=s.device) if need_w else None
     db = torch.empty(bias.shape, dtype=bias.dtype, device=s.device) if need_b else None
-    part = torch.empty(L.kfac_ln_ws_floats(rows, D), dtype=torch.float32, device=s.device) \
+    part = torch.empty(L.kfac_ln_ws_floats(_code(s), rows, D), dtype=torch.float32, device=s.device) \
         if need_w or need_b else None
     w = None if weight is None else weight.contiguous()
     with _lib.device_guard(s.device):

@@ -14,7 +14,29 @@
 // chunks in order: no atomics, bitwise reproducible.
 #include "rows.h"
 
+// argument records (ops/ln.py packs the same fields); chunks is set here
+struct KfacLnFwd {
+  const void *x, *z, *w, *b;
+  void *y, *s;
+  float *mean, *rstd;
+  long long ldx, ldz, rows, D;
+  int sdt, zdt, wdt, bdt, ydt;
+  float eps;
+};
+
+struct KfacLnBwd {
+  const void *dy, *ds, *s, *w;
+  const float *mean, *rstd;
+  void *dx, *dz, *dw, *db;
+  float* part;
+  long long lddy, ldds, lds, rows, D;
+  int sdt, zdt, wdt, bdt, ydt, chunks;
+};
+
 namespace {
+
+typedef KfacLnFwd Fwd;
+typedef KfacLnBwd Bwd;
 
 constexpr int NT = 256;
 
@@ -38,15 +60,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   for (int i = 1; i < NT / 64; ++i) r += red[i];
   return r;
 }
-
-struct Fwd {
-  const void *x, *z, *w, *b;
-  void *y, *s;
-  float *mean, *rstd;
-  long long ldx, ldz, rows, D;
-  int sdt, zdt, wdt, bdt, ydt;
-  float eps;
-};
 
 __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const Fwd a) {
   __shared__ float red[NT / 64];
@@ -82,15 +95,6 @@ __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const Fwd a) {
     a.rstd[row] = rstd;
   }
 }
-
-struct Bwd {
-  const void *dy, *ds, *s, *w;
-  const float *mean, *rstd;
-  void *dx, *dz, *dw, *db;
-  float* part;
-  long long lddy, ldds, lds, rows, D;
-  int sdt, zdt, wdt, bdt, ydt, chunks;
-};
 
 __global__ __launch_bounds__(NT) void ln_bwd_long_kernel(const Bwd a) {
   __shared__ float red[NT / 64];
@@ -473,22 +477,21 @@ KFAC_API long long kfac_ln_ws_floats(int sdt, long long rows, long long D) {
   return 2LL * param_chunks(sdt, rows, D) * D;
 }
 
-// z and s null: the norm of x.  w, b may be null; mean, rstd (fp32, one a row)
-// may be null where no backward pass follows.
-KFAC_API int kfac_ln_forward(const void* x, long long ldx, int sdt, const void* z, long long ldz,
-                             int zdt, const void* w, int wdt, const void* b, int bdt, void* y,
-                             int ydt, void* s, float* mean, float* rstd, long long rows,
-                             long long D, float eps, hipStream_t stream) {
-  if (rows <= 0 || rows > 0x7fffffffLL || D <= 0 || !dtype_ok(sdt) || !dtype_ok(ydt) ||
-      (z && (!s || !dtype_ok(zdt))) || (w && !dtype_ok(wdt)) || (b && !dtype_ok(bdt)) ||
-      !mean != !rstd)
+// The argument record of ops/ln.py (`bytes`: its size there).  z and s null:
+// the norm of x.  w, b may be null; mean, rstd (fp32, one a row) may be null
+// where no backward pass follows.
+KFAC_API int kfac_ln_forward(const KfacLnFwd* args, int bytes, hipStream_t stream) {
+  if (bytes != (int)sizeof(KfacLnFwd)) return -2;
+  const Fwd a = *args;
+  if (!a.x || !a.y || a.rows <= 0 || a.rows > 0x7fffffffLL || a.D <= 0 || !dtype_ok(a.sdt) ||
+      !dtype_ok(a.ydt) || (a.z && (!a.s || !dtype_ok(a.zdt))) || (a.w && !dtype_ok(a.wdt)) ||
+      (a.b && !dtype_ok(a.bdt)) || !a.mean != !a.rstd)
     return -2;
-  Fwd a = {x, z, w, b, y, s, mean, rstd, ldx, ldz, rows, D, sdt, zdt, wdt, bdt, ydt, eps};
-  if (looped(sdt, D))
-    hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
-  else if (sdt == KDT_F32)
+  if (looped(a.sdt, a.D))
+    hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)a.rows), dim3(NT), 0, stream, a);
+  else if (a.sdt == KDT_F32)
     launch_fwd_any<KDT_F32>(a, stream);
-  else if (sdt == KDT_BF16)
+  else if (a.sdt == KDT_BF16)
     launch_fwd_any<KDT_BF16>(a, stream);
   else
     launch_fwd_any<KDT_F16>(a, stream);
@@ -497,31 +500,30 @@ KFAC_API int kfac_ln_forward(const void* x, long long ldx, int sdt, const void* 
 
 // ds (the gradient that reaches s itself), dx, dz, dw, db may be null; part
 // (kfac_ln_ws_floats) is needed where dw or db is asked for
-KFAC_API int kfac_ln_backward(const void* dy, long long lddy, int ydt, const void* ds,
-                              long long ldds, const void* s, long long lds, int sdt,
-                              const void* w, int wdt, int bdt, const float* mean,
-                              const float* rstd, void* dx, void* dz, int zdt, void* dw, void* db,
-                              float* part, long long rows, long long D, hipStream_t stream) {
-  if (rows <= 0 || rows > 0x7fffffffLL || D <= 0 || !dtype_ok(sdt) || !dtype_ok(ydt) ||
-      (dz && (!dx || !dtype_ok(zdt))) || ((w || dw) && !dtype_ok(wdt)) ||
-      (db && !dtype_ok(bdt)) || ((dw || db) && !part))
+KFAC_API int kfac_ln_backward(const KfacLnBwd* args, int bytes, hipStream_t stream) {
+  if (bytes != (int)sizeof(KfacLnBwd)) return -2;
+  Bwd a = *args;
+  if (!a.dy || !a.s || !a.mean || !a.rstd || a.rows <= 0 || a.rows > 0x7fffffffLL || a.D <= 0 ||
+      !dtype_ok(a.sdt) || !dtype_ok(a.ydt) || (a.dz && (!a.dx || !dtype_ok(a.zdt))) ||
+      ((a.w || a.dw) && !dtype_ok(a.wdt)) || (a.db && !dtype_ok(a.bdt)) ||
+      ((a.dw || a.db) && !a.part))
     return -2;
-  Bwd a = {dy, ds, s, w, mean, rstd, dx, dz, dw, db, dw || db ? part : nullptr, lddy, ldds, lds,
-           rows, D, sdt, zdt, wdt, bdt, ydt, param_chunks(sdt, rows, D)};
-  if (looped(sdt, D)) {
-    if (dx) hipLaunchKernelGGL(ln_bwd_long_kernel, dim3((unsigned)rows), dim3(NT), 0, stream, a);
+  if (!a.dw && !a.db) a.part = nullptr;
+  a.chunks = param_chunks(a.sdt, a.rows, a.D);
+  if (looped(a.sdt, a.D)) {
+    if (a.dx) hipLaunchKernelGGL(ln_bwd_long_kernel, dim3((unsigned)a.rows), dim3(NT), 0, stream, a);
     if (a.part)
-      hipLaunchKernelGGL(ln_param_part_kernel, dim3((unsigned)((D + NT - 1) / NT), a.chunks),
+      hipLaunchKernelGGL(ln_param_part_kernel, dim3((unsigned)((a.D + NT - 1) / NT), a.chunks),
                          dim3(NT), 0, stream, a);
-  } else if (sdt == KDT_F32) {
+  } else if (a.sdt == KDT_F32) {
     launch_bwd_any<KDT_F32>(a, stream);
-  } else if (sdt == KDT_BF16) {
+  } else if (a.sdt == KDT_BF16) {
     launch_bwd_any<KDT_BF16>(a, stream);
   } else {
     launch_bwd_any<KDT_F16>(a, stream);
   }
   if (a.part)
-    hipLaunchKernelGGL(ln_param_sum_kernel, dim3((unsigned)((D + 31) / 32)), dim3(1024), 0,
+    hipLaunchKernelGGL(ln_param_sum_kernel, dim3((unsigned)((a.D + 31) / 32)), dim3(1024), 0,
                        stream, a);
   return (int)hipGetLastError();
 }

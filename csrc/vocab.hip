@@ -13,17 +13,69 @@
 // the type's lowest value).  Subtracting M before the division by T keeps
 // every finite row finite.
 //
+// Forward: ONE pass over the row.  A thread keeps the running maximum m of its
+// elements, s = sum exp((x - m) / T) and a = sum exp((x - m) / T) (x - m), each
+// brought to a new maximum once per tile of four 16-byte loads; the threads'
+// (m, s, a) are joined at the end.  The alternatives need no second pass: the
+// k-th largest of the threads' maxima is a bound that at least k elements
+// reach, and only the threads that reach it have such elements, so about k of
+// 256 threads' elements are looked at again.  A row is cut over several
+// workgroups where there are few rows, and joined by a second kernel.
+// Backward: one read and one write of the row from the saved (M, L).
+//
 // Defined edges: a row whose target is `ignore` is neither read nor gives a
 // gradient (0, ids -1); a row of only -inf has logprob -inf, entropy 0 and no
 // gradient; NaN or +inf in a row, or a target out of range, makes its results
 // NaN; a teacher row without a used slot (id -1) or with only -inf gives
 // loss 0 and no gradient.
-#include "common.h"
+#include "rows.h"
+
+// argument records (ops/vocab.py packs the same fields)
+struct KfacVocabFwd {
+  const void* x;
+  const long long* targets;
+  float *logprob, *entropy, *top_lp;
+  long long* top_ids;
+  float* stats;                   // (M, L) a row
+  const long long* ids;           // teacher
+  const void* teacher;
+  float* loss;
+  int* keep_ids;                  // ids (each once) and masses for the backward pass
+  float* keep_q;
+  void* ws;
+  long long ld, rows, V, ignore;
+  int dt, k, K, tdt;
+  float inv_t;
+};
+
+struct KfacVocabBwd {
+  const void* x;
+  const float *stats, *entropy;
+  const long long* targets;
+  const float *g, *gh;
+  const int* keep_ids;
+  const float* keep_q;
+  void* dx;
+  long long ld, rows, V, ignore, gs, ghs;
+  int dt, K;
+  float inv_t;
+};
 
 namespace {
 
-constexpr int NT = 256;
-constexpr int TOP_MAX = 128;      // alternatives a row: at most one a thread
+typedef KfacVocabFwd Fwd;
+typedef KfacVocabBwd Bwd;
+
+
+constexpr int TOP_MAX = 128;      // alternatives, and slots of a teacher's row
+constexpr int MAX_V = 1 << 30;    // elements of a row: 32-bit offsets within it
+constexpr int MAX_SPLITS = 64;    // workgroups a row
+constexpr float LOG2E = 1.4426950408889634f;
+// A distance to the maximum below which exp(d / T) is 0 for every T <= 1e4 that
+// the operators take; a product 0 d stays 0 when d is no lower than this.
+constexpr float LOWEST = -1e9f;
+
+enum Mode { LOGPROB = 0, DISTILL = 1 };
 
 // order of a value as an unsigned number: -inf lowest, NaN highest, -0 as +0;
 // 0 itself is no value's
@@ -32,97 +84,401 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
 // unique a row: larger value first, then the lower index
 __device__ __forceinline__ uint64_t full_key(float v, uint32_t i) {
   return ((uint64_t)order_key(v) << 32) | (uint32_t)~i;
 }
 
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = wave_sum(v);
-  __syncthreads();                       // red may still be read from the last call
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = red[0];
-  for (int i = 1; i < NT / 64; ++i) r += red[i];
-  return r;
-}
-__device__ __forceinline__ float block_max(float v, float* red) {
-  for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = red[0];
-  for (int i = 1; i < NT / 64; ++i) r = fmaxf(r, red[i]);
-  return r;
-}
-__device__ __forceinline__ uint64_t block_max_key(uint64_t v, uint64_t* red) {
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor((unsigned long long)v, o, 64);
-    v = u > v ? u : v;
+// One workgroup of NT threads: reductions to every thread, in a fixed order.
+template <int NT> struct Group {
+  static __device__ __forceinline__ float sum(float v, float* red) {
+    v = wave_sum(v);
+    if (NT <= 64) return v;
+    __syncthreads();                     // red may still be read from the last call
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) r += red[i];
+    return r;
   }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  uint64_t r = red[0];
-  for (int i = 1; i < NT / 64; ++i) r = red[i] > r ? red[i] : r;
-  return r;
-}
+  static __device__ __forceinline__ float max(float v, float* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if (NT <= 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float r = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) r = fmaxf(r, red[i]);
+    return r;
+  }
+};
 
 // lp_i; -inf in a row of only -inf
 __device__ __forceinline__ float log_prob(float x, float M, float L, float inv_t) {
   return M == -INFINITY ? -INFINITY : (x - M) * inv_t - L;
 }
 
-struct Row {
-  const void* x;
-  long long ld, rows, V;
-  float inv_t;
-};
+// A part of a row: what one of the `splits` workgroups of a row hands on.
+struct Part { float m, s, a, pad; };
 
-// M, L and sum exp(d) d / sum exp(d) of a row, d = (x - M) / T
+// Elements i .. i + V - 1 of a row of n, -inf from `end` on.
 template <int DT>
-__device__ __forceinline__ void row_stats(const typename DTypeTraits<DT>::raw_t* x, long long V,
-                                          float inv_t, float* red, float& M, float& L, float& t) {
-  float m = -INFINITY;
-  for (long long i = threadIdx.x; i < V; i += NT) m = fmaxf(m, DTypeTraits<DT>::to_f32(x[i]));
-  M = block_max(m, red);
-  const float base = M == -INFINITY ? 0.f : M;
-  float s = 0.f, a = 0.f;
-  for (long long i = threadIdx.x; i < V; i += NT) {
-    const float d = (DTypeTraits<DT>::to_f32(x[i]) - base) * inv_t;
-    const float e = __expf(d);
-    s += e;
-    a = fmaf(e, fmaxf(d, -1e30f), a);    // exp(-inf) = 0 times a finite number
+__device__ __forceinline__ void fetch(const AS1 typename DTypeTraits<DT>::raw_t* x, int i, int end,
+                                      int n, float* f) {
+  constexpr int V = row_vec<DT>();
+  if (n < V) {                           // no 16 bytes in the whole row
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = i + e < end ? DTypeTraits<DT>::to_f32(x[i + e]) : -INFINITY;
+    return;
   }
-  s = block_sum(s, red);
-  a = block_sum(a, red);
-  L = logf(s);
-  t = a / s;
+  vec_to_f32<DT>(clip_vec<DT, true>(load_vec<DT, true>(x, i, n), i, n), f);
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (i + e >= end) f[e] = -INFINITY;
 }
 
-struct LogprobArgs {
-  Row r;
-  const long long* targets;
-  long long ignore;
-  float *logprob, *entropy, *top_lp, *stats;
-  long long* top_ids;
-  int k;
+// The running (m, s, a) of one thread over a tile of N elements.
+template <int N, bool ENT>
+__device__ __forceinline__ void fold(const float* f, float c1, float& m, float& s, float& a) {
+  float top = m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) top = fmaxf(top, f[e]);
+  const float base = top == -INFINITY ? 0.f : top;
+  const float back = fmaxf(m - base, LOWEST), scale = __builtin_amdgcn_exp2f(back * c1);
+  if (ENT) a = scale * fmaf(back, s, a);
+  s *= scale;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float d = f[e] - base, x = __builtin_amdgcn_exp2f(d * c1);
+    s += x;
+    if (ENT) a = fmaf(x, fmaxf(d, LOWEST), a);      // exp(-inf) = 0 times a finite number
+  }
+  m = top;
+}
+
+template <int DT, int NT, bool ENT>
+__device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* x, int begin,
+                                     int end, int n, float c1, float& m, float& s, float& a) {
+  constexpr int V = row_vec<DT>(), U = 4, STEP = NT * V;
+  m = -INFINITY;
+  s = a = 0.f;
+  int at = begin;
+  for (; at + U * STEP <= end; at += U * STEP) {
+    const int i = at + threadIdx.x * V;
+    u32x4n raw[U];
+    float f[U * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = *(const AS1 u32x4u*)(x + i + u * STEP);
+#pragma unroll
+    for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
+    fold<U * V, ENT>(f, c1, m, s, a);
+  }
+  if (at < end) {
+    const int i = at + threadIdx.x * V;
+    float f[U * V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch<DT>(x, i + u * STEP, end, n, f + u * V);
+    fold<U * V, ENT>(f, c1, m, s, a);
+  }
+}
+
+// (m, s, a) joined over the workgroup
+template <int NT, bool ENT>
+__device__ __forceinline__ void join(float c1, float* red, float& m, float& s, float& a) {
+  const float M = Group<NT>::max(m, red), base = M == -INFINITY ? 0.f : M;
+  const float back = fmaxf(m - base, LOWEST), scale = __builtin_amdgcn_exp2f(back * c1);
+  if (ENT) a = Group<NT>::sum(scale * fmaf(back, s, a), red);
+  s = Group<NT>::sum(s * scale, red);
+  m = M;
+}
+
+// The threads that hold elements are fewer than k only where the chunk is one
+// access a thread: then all its elements, at most k V of them, are candidates.
+template <int NT> struct TopShared {
+  static constexpr int CAND = 4 * NT;
+  uint64_t cand[CAND];
+  uint32_t key[NT];
+  int list[NT];
+  int hist[256];
+  int n, winners, bound;
 };
 
-template <int DT>
-__global__ __launch_bounds__(NT) void logprob_fwd_kernel(const LogprobArgs a) {
+// The k largest (value, lower index) of a chunk of a row as full keys, largest
+// first, handed to out(rank, key); fewer than k elements give fewer.  m, s: the
+// calling thread's running maximum and sum.
+template <int DT, int NT, class Out>
+__device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>::raw_t* x,
+                                             int begin, int end, int n, float m, float s, int k,
+                                             TopShared<NT>& sh, Out out) {
+  constexpr int V = row_vec<DT>(), STEP = NT * V;
+  // low bits of a key that say nothing: bf16 fills 16 bits of an fp32, fp16 19
+  constexpr int LOW = DT == KDT_F32 ? 0 : DT == KDT_BF16 ? 16 : 8;
+  const int tid = threadIdx.x, mine = begin + tid * V, per = (end - begin + STEP - 1) / STEP;
+  // this thread's largest key; a NaN or +inf made s NaN, the maximum passes over NaN
+  uint32_t key = mine < end ? order_key(m) : 0u;
+  if (s != s) {
+    key = 0;
+    for (int j = 0; j < per; ++j) {
+      float f[V];
+      const int i = mine + j * STEP;
+      if (i >= end) break;
+      fetch<DT>(x, i, end, n, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint32_t o = i + e < end ? order_key(f[e]) : 0u;
+        key = o > key ? o : key;
+      }
+    }
+  }
+  sh.key[tid] = key;
+  if (tid == 0) sh.n = sh.winners = 0;
+  __syncthreads();
+  // the k-th largest of the threads' keys, bit by bit (0 where there are fewer)
+  if (tid < 64) {
+    uint32_t own[NT / 64], bound = 0;
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j) own[j] = sh.key[tid + 64 * j];
+    for (int bit = 31; bit >= LOW; --bit) {
+      const uint32_t next = bound | 1u << bit;
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < NT / 64; ++j) count += __popcll(__ballot(own[j] >= next));
+      if (count >= k) bound = next;
+    }
+    if (tid == 0) sh.bound = (int)bound;
+  }
+  __syncthreads();
+  const uint32_t bound = (uint32_t)sh.bound ? (uint32_t)sh.bound : 1u;
+  if (key >= bound) sh.list[atomicAdd(&sh.winners, 1)] = tid;
+  __syncthreads();
+  const int items = sh.winners * per;
+  for (int it = tid; it < items; it += NT) {
+    const int w = it / per, i = begin + sh.list[w] * V + (it - w * per) * STEP;
+    if (i >= end) continue;
+    float f[V];
+    fetch<DT>(x, i, end, n, f);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (i + e < end && order_key(f[e]) >= bound) {
+        const int c = atomicAdd(&sh.n, 1);
+        if (c < TopShared<NT>::CAND) sh.cand[c] = full_key(f[e], (uint32_t)(i + e));
+      }
+  }
+  __syncthreads();
+  if (sh.n > TopShared<NT>::CAND) {
+    // Too many equal or crowded values: the k-th largest key exactly, by counting
+    // its digits from the top; then the larger ones and, in the order of their
+    // indices, as many equal ones as are wanted -- k in all.
+    int need = k;
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= LOW; shift -= 8) {
+      for (int j = tid; j < 256; j += NT) sh.hist[j] = 0;
+      __syncthreads();
+      for (int j = 0; j < per; ++j) {
+        float f[V];
+        const int i = mine + j * STEP;
+        if (i >= end) break;
+        fetch<DT>(x, i, end, n, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const uint32_t o = order_key(f[e]);
+          if (i + e < end && (uint64_t)o >> (shift + 8) == prefix)
+            atomicAdd(&sh.hist[(o >> shift) & 255], 1);
+        }
+      }
+      __syncthreads();
+      int digit = 255, left = need;
+      while (digit > 0 && sh.hist[digit] < left) left -= sh.hist[digit--];
+      need = left;
+      prefix = prefix << 8 | (uint32_t)digit;
+      __syncthreads();
+    }
+    const uint32_t low = LOW ? (1u << LOW) - 1u : 0u, kth = prefix << LOW;   // of the digits counted
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    for (int j = 0; j < per; ++j) {
+      float f[V];
+      const int i = mine + j * STEP;
+      if (i >= end) break;
+      fetch<DT>(x, i, end, n, f);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i + e < end && order_key(f[e]) > (kth | low))
+          sh.cand[atomicAdd(&sh.n, 1)] = full_key(f[e], (uint32_t)(i + e));
+    }
+    __syncthreads();
+    int have = sh.n;                       // k - need
+    for (int at = begin; at < end && have < k; at += STEP) {
+      float f[V];
+      const int i = at + tid * V;
+      int mine_n = 0;
+      if (i < end) {
+        fetch<DT>(x, i, end, n, f);
+#pragma unroll
+        for (int e = 0; e < V; ++e) mine_n += i + e < end && (order_key(f[e]) | low) == (kth | low);
+      }
+      __syncthreads();
+      sh.list[tid] = mine_n;
+      __syncthreads();
+      int before = have, all = have;
+      for (int j = 0; j < NT; ++j) {
+        before += j < tid ? sh.list[j] : 0;
+        all += sh.list[j];
+      }
+      if (mine_n) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (i + e < end && (order_key(f[e]) | low) == (kth | low)) {
+            if (before < k) sh.cand[before] = full_key(f[e], (uint32_t)(i + e));
+            ++before;
+          }
+      }
+      have = all;
+    }
+    __syncthreads();
+    if (tid == 0) sh.n = k;
+    __syncthreads();
+  }
+  const int count = sh.n;
+  for (int c = tid; c < count; c += NT) {
+    const uint64_t v = sh.cand[c];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += sh.cand[j] > v;
+    if (rank < k) out(rank, v);
+  }
+}
+
+__device__ __forceinline__ float any_value(const void* t, long long i, int dt) {
+  if (dt == KDT_F32) return ((const float*)t)[i];
+  const uint16_t v = ((const uint16_t*)t)[i];
+  return dt == KDT_BF16 ? bf16_bits_to_f32(v) : f16_bits_to_f32(v);
+}
+
+struct SlotShared {
+  int id[TOP_MAX];
+  float q[TOP_MAX];
+};
+
+// The teacher's side of a row, and the loss, from the student's (M, L).
+template <int DT, int NT>
+__device__ __forceinline__ void distill_row(const Fwd& a, long long row, float M, float L,
+                                            SlotShared& sh, float* red) {
+  const AS1 typename DTypeTraits<DT>::raw_t* x =
+      gptr((const typename DTypeTraits<DT>::raw_t*)a.x) + row * a.ld;
+  constexpr int P = (TOP_MAX + NT - 1) / NT;       // slots a thread
+  int id[P];
+  float t[P], top = -INFINITY;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int j = threadIdx.x + p * NT;
+    const long long v = j < a.K ? a.ids[row * a.K + j] : -1;
+    t[p] = v == -1 ? -INFINITY : any_value(a.teacher, row * a.K + j, a.tdt);
+    if (v < -1 || v >= a.V) t[p] = NAN;            // makes the row's sum NaN
+    id[p] = v < 0 || v >= a.V ? -1 : (int)v;
+    top = fmaxf(top, t[p]);
+  }
+  top = Group<NT>::max(top, red);
+  if (top == -INFINITY) top = 0.f;                 // only -inf and NaN
+  float z = 0.f;
+#pragma unroll
+  for (int p = 0; p < P; ++p) z += __builtin_amdgcn_exp2f((t[p] - top) * a.inv_t * LOG2E);
+  z = Group<NT>::sum(z, red);
+  const float logz = logf(z);
+  float term = 0.f, q[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const float d = (t[p] - top) * a.inv_t;
+    q[p] = __builtin_amdgcn_exp2f(d * LOG2E) / z;
+    const int j = threadIdx.x + p * NT;
+    if (j < a.K && q[p] != 0.f) {
+      const float lp = id[p] < 0 ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[id[p]]), M, L, a.inv_t);
+      term += q[p] * (d - logz - lp);
+    }
+    if (j < TOP_MAX) {
+      sh.id[j] = id[p];
+      sh.q[j] = q[p];
+    }
+  }
+  term = Group<NT>::sum(term, red);
+  if (threadIdx.x == 0) {
+    a.loss[row] = term;
+    a.stats[2 * row] = M;
+    a.stats[2 * row + 1] = z == z ? L : NAN;       // NaN all along the gradient's row
+  }
+  __syncthreads();
+  // the same id twice: its masses are added in slot order, into its first slot
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int j = threadIdx.x + p * NT;
+    if (j >= a.K) break;
+    float mass = 0.f;
+    bool first = true;
+    for (int o = 0; o < a.K; ++o)
+      if (sh.id[o] == id[p]) {
+        if (o < j) first = false;
+        mass += sh.q[o];
+      }
+    a.keep_ids[row * a.K + j] = first ? id[p] : -1;
+    a.keep_q[row * a.K + j] = mass;
+  }
+}
+
+// whether a row of slots has any mass
+template <int NT>
+__device__ __forceinline__ bool has_teacher(const Fwd& a, long long row, float* red) {
+  float any = 0.f;
+  for (int j = threadIdx.x; j < a.K; j += NT)
+    if (a.ids[row * a.K + j] != -1) {
+      const long long v = a.ids[row * a.K + j];
+      const float t = any_value(a.teacher, row * a.K + j, a.tdt);
+      if (t != -INFINITY || v < -1 || v >= a.V) any = 1.f;
+    }
+  return Group<NT>::max(any, red) > 0.f;
+}
+
+template <int DT, int NT>
+__device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M, float s,
+                                            float sum, float& L) {
+  L = logf(s);
+  if (threadIdx.x != 0) return;
+  const AS1 typename DTypeTraits<DT>::raw_t* x =
+      gptr((const typename DTypeTraits<DT>::raw_t*)a.x) + row * a.ld;
+  if (a.logprob) {
+    const long long t = a.targets[row];
+    a.logprob[row] =
+        t < 0 || t >= a.V ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[t]), M, L, a.inv_t);
+  }
+  if (a.entropy) a.entropy[row] = M == -INFINITY ? 0.f : L - sum / s * a.inv_t;
+  a.stats[2 * row] = M;
+  a.stats[2 * row + 1] = L;
+}
+
+template <int DT, int NT, int MODE, bool ENT, bool TOP>
+__global__ __launch_bounds__(NT) void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
   __shared__ float red[NT / 64];
-  __shared__ uint64_t redk[NT / 64];
-  const long long row = blockIdx.x;
-  const raw_t* x = (const raw_t*)a.r.x + row * a.r.ld;
-  const long long tgt = a.targets ? a.targets[row] : 0;
-  if (a.targets && tgt == a.ignore) {
-    if (threadIdx.x < a.k) {
-      a.top_lp[row * a.k + threadIdx.x] = -INFINITY;
-      a.top_ids[row * a.k + threadIdx.x] = -1;
-    }
+  __shared__ TopShared<TOP ? NT : 1> tops;
+  const long long row = blockIdx.x / splits;
+  const int part = blockIdx.x % splits, n = (int)a.V;
+  const int begin = part * chunk, end = n - begin < chunk ? n : begin + chunk;
+  const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ld;
+  const bool skip = MODE == DISTILL ? !has_teacher<NT>(a, row, red)
+                                    : a.targets && a.targets[row] == a.ignore;
+  if (skip) {
+    if (part != 0) return;
+    if (TOP)
+      for (int j = threadIdx.x; j < a.k; j += NT) {
+        a.top_lp[row * a.k + j] = -INFINITY;
+        a.top_ids[row * a.k + j] = -1;
+      }
     if (threadIdx.x == 0) {
+      if (a.loss) a.loss[row] = 0.f;
       if (a.logprob) a.logprob[row] = 0.f;
       if (a.entropy) a.entropy[row] = 0.f;
       a.stats[2 * row] = -INFINITY;
@@ -130,251 +486,281 @@ __global__ __launch_bounds__(NT) void logprob_fwd_kernel(const LogprobArgs a) {
     }
     return;
   }
-  float M, L, t;
-  row_stats<DT>(x, a.r.V, a.r.inv_t, red, M, L, t);
-  if (threadIdx.x == 0) {
-    const bool bad = tgt < 0 || tgt >= a.r.V;
-    if (a.logprob)
-      a.logprob[row] = bad ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[tgt]), M, L, a.r.inv_t);
-    if (a.entropy) a.entropy[row] = M == -INFINITY ? 0.f : L - t;
-    a.stats[2 * row] = M;
-    a.stats[2 * row + 1] = L;
-  }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < a.k; ++j) {
-    uint64_t best = 0;
-    for (long long i = threadIdx.x; i < a.r.V; i += NT) {
-      const uint64_t key = full_key(DTypeTraits<DT>::to_f32(x[i]), (uint32_t)i);
-      if (key < last && key > best) best = key;
-    }
-    last = block_max_key(best, redk);
-    if (threadIdx.x == 0) {
-      const long long id = (uint32_t)~(uint32_t)last;
-      a.top_ids[row * a.k + j] = id;
-      a.top_lp[row * a.k + j] = log_prob(DTypeTraits<DT>::to_f32(x[id]), M, L, a.r.inv_t);
-    }
-  }
-}
-
-struct LogprobBwd {
-  Row r;
-  const long long* targets;
-  long long ignore;
-  const float *stats, *entropy, *g, *gh;
-  long long gs, ghs;
-  void* dx;
-};
-
-template <int DT>
-__global__ __launch_bounds__(NT) void logprob_bwd_kernel(const LogprobBwd a) {
-  typedef typename DTypeTraits<DT>::raw_t raw_t;
-  const long long row = blockIdx.x, V = a.r.V;
-  const raw_t* x = (const raw_t*)a.r.x + row * a.r.ld;
-  raw_t* dx = (raw_t*)a.dx + row * V;
-  const long long tgt = a.targets ? a.targets[row] : 0;
-  const float M = a.stats[2 * row], L = a.stats[2 * row + 1];
-  const bool zero = (a.targets && tgt == a.ignore) || M == -INFINITY;
-  float g = a.g ? a.g[row * a.gs] : 0.f;
-  if (a.g && (tgt < 0 || tgt >= V)) g = NAN;
-  const float gh = a.gh ? a.gh[row * a.ghs] : 0.f, H = a.gh ? a.entropy[row] : 0.f;
-  for (long long i = threadIdx.x; i < V; i += NT) {
-    float v = 0.f;
-    if (!zero) {
-      const float lp = (DTypeTraits<DT>::to_f32(x[i]) - M) * a.r.inv_t - L;
-      v = -__expf(lp) * (g + gh * (fmaxf(lp, -1e30f) + H));
-      if (a.g && i == tgt) v += g;
-      v *= a.r.inv_t;
-    }
-    dx[i] = DTypeTraits<DT>::from_f32(v);
-  }
-}
-
-// The teacher's side of a row: slot j in thread j.  Returns false for a row
-// without a used slot (or with only -inf); q, log q of the thread's slot
-// (0, -inf for an unused one).  bad: an id out of range, or NaN.
-__device__ __forceinline__ float teacher_value(const void* t, long long i, int dt) {
-  if (dt == KDT_F32) return ((const float*)t)[i];
-  const uint16_t v = ((const uint16_t*)t)[i];
-  return dt == KDT_BF16 ? bf16_bits_to_f32(v) : f16_bits_to_f32(v);
-}
-
-struct Teacher {
-  const long long* ids;
-  const void* t;
-  int dt, K;
-};
-
-__device__ __forceinline__ bool teacher_row(const Teacher& h, long long row, long long V,
-                                            float inv_t, float* red, long long& id, float& q,
-                                            float& logq) {
-  const int j = threadIdx.x;
-  id = j < h.K ? h.ids[row * h.K + j] : -1;
-  float t = id == -1 ? -INFINITY : teacher_value(h.t, row * h.K + j, h.dt);
-  if (id < -1 || id >= V) { t = NAN; id = -1; }
-  const float top = block_max(t, red);
-  const float nan = block_sum(t != t ? 1.f : 0.f, red);
-  if (top == -INFINITY && nan == 0.f) return false;
-  const float d = (t - top) * inv_t;
-  const float Z = block_sum(__expf(d), red);
-  q = __expf(d) / Z;
-  logq = d - logf(Z);
-  return true;
-}
-
-struct DistillArgs {
-  Row r;
-  Teacher h;
-  float *loss, *stats;
-};
-
-template <int DT>
-__global__ __launch_bounds__(NT) void distill_fwd_kernel(const DistillArgs a) {
-  typedef typename DTypeTraits<DT>::raw_t raw_t;
-  __shared__ float red[NT / 64];
-  const long long row = blockIdx.x;
-  const raw_t* x = (const raw_t*)a.r.x + row * a.r.ld;
-  long long id;
-  float q, logq, M, L, t;
-  if (!teacher_row(a.h, row, a.r.V, a.r.inv_t, red, id, q, logq)) {
-    if (threadIdx.x == 0) {
-      a.loss[row] = 0.f;
-      a.stats[2 * row] = -INFINITY;
-      a.stats[2 * row + 1] = 0.f;
+  const float c1 = a.inv_t * LOG2E;
+  float m, s, sum;
+  scan<DT, NT, ENT>(x, begin, end, n, c1, m, s, sum);
+  float M = m, S = s;
+  join<NT, ENT>(c1, red, M, S, sum);
+  if (splits > 1) {
+    Part* p = (Part*)a.ws + row * splits + part;
+    if (threadIdx.x == 0) *p = Part{M, S, sum, 0.f};
+    if constexpr (TOP) {
+      uint64_t* keys = (uint64_t*)((Part*)a.ws + a.rows * splits) + (row * splits + part) * a.k;
+      for (int j = threadIdx.x; j < a.k; j += NT)
+        if (j >= end - begin) keys[j] = 0;         // fewer elements than k
+      top_of_chunk<DT, NT>(x, begin, end, n, m, s, a.k, tops,
+                           [&](int rank, uint64_t key) { keys[rank] = key; });
     }
     return;
   }
-  row_stats<DT>(x, a.r.V, a.r.inv_t, red, M, L, t);
-  float term = 0.f;
-  if (q != 0.f)
-    term = q * (logq - (id < 0 ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[id]), M, L, a.r.inv_t)));
-  term = block_sum(term, red);
-  if (threadIdx.x == 0) {
-    a.loss[row] = term;
-    a.stats[2 * row] = M;
-    a.stats[2 * row + 1] = L;
-  }
-}
-
-struct DistillBwd {
-  Row r;
-  Teacher h;
-  const float *stats, *g;
-  long long gs;
-  void* dx;
-};
-
-template <int DT>
-__global__ __launch_bounds__(NT) void distill_bwd_kernel(const DistillBwd a) {
-  typedef typename DTypeTraits<DT>::raw_t raw_t;
-  __shared__ float red[NT / 64];
-  __shared__ long long ids[TOP_MAX];
-  __shared__ float qs[TOP_MAX];
-  const long long row = blockIdx.x, V = a.r.V;
-  const raw_t* x = (const raw_t*)a.r.x + row * a.r.ld;
-  raw_t* dx = (raw_t*)a.dx + row * V;
-  long long id;
-  float q = 0.f, logq;
-  const bool some = teacher_row(a.h, row, V, a.r.inv_t, red, id, q, logq);
-  const float M = a.stats[2 * row], L = a.stats[2 * row + 1];
-  const bool zero = !some || M == -INFINITY;
-  const float g = a.g[row * a.gs] * a.r.inv_t;
-  // an id out of range or NaN in the teacher's row made every q NaN
-  const float all = some && block_sum(q, red) != block_sum(q, red) ? NAN : 1.f;
-  for (long long i = threadIdx.x; i < V; i += NT) {
-    float v = 0.f;
-    if (!zero) v = g * all * __expf((DTypeTraits<DT>::to_f32(x[i]) - M) * a.r.inv_t - L);
-    dx[i] = DTypeTraits<DT>::from_f32(v);
-  }
-  if (zero) return;
-  if (threadIdx.x < a.h.K) {
-    ids[threadIdx.x] = id;
-    qs[threadIdx.x] = q;
-  }
-  __syncthreads();                       // dx of the row is written, too
-  if (threadIdx.x < a.h.K && id >= 0) {
-    // the same id twice: its masses are added in slot order, by its first slot
-    float sum = 0.f;
-    bool first = true;
-    for (int j = 0; j < a.h.K; ++j)
-      if (ids[j] == id) {
-        if (j < (int)threadIdx.x) first = false;
-        sum += qs[j];
-      }
-    if (first) {
-      const float p = __expf((DTypeTraits<DT>::to_f32(x[id]) - M) * a.r.inv_t - L);
-      dx[id] = DTypeTraits<DT>::from_f32(g * (p - sum));
+  if constexpr (MODE == DISTILL) {
+    __shared__ SlotShared slots;
+    distill_row<DT, NT>(a, row, M, logf(S), slots, red);
+  } else {
+    float L;
+    logprob_row<DT, NT>(a, row, M, S, sum, L);
+    if constexpr (TOP) {
+      top_of_chunk<DT, NT>(x, begin, end, n, m, s, a.k, tops, [&](int rank, uint64_t key) {
+        a.top_ids[row * a.k + rank] = (uint32_t)~(uint32_t)key;
+        a.top_lp[row * a.k + rank] = log_prob(key_value((uint32_t)(key >> 32)), M, L, a.inv_t);
+      });
     }
   }
 }
 
-bool row_ok(const Row& r, int dt) {
-  return r.x && r.rows > 0 && r.rows <= 0x7fffffffLL && r.V > 0 && r.V <= 0x7fffffffLL &&
-         r.inv_t > 0.f && (dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16);
+// Joins the parts of a row.  The alternatives: every part has its own k largest
+// in order; with j of a part's keys at least as large as the r-th largest of
+// all parts' j-th keys, r j >= k, that key is a bound which at least k keys
+// reach and no more than r k + splits j.
+constexpr int JOIN_NT = 256;
+constexpr int JOIN_CAND = 2560;
+
+__host__ __device__ constexpr int join_depth(int k, int splits) {
+  const int j = (4 * k + splits - 1) / splits;
+  return j < k ? j : k;
 }
-bool teacher_ok(const Teacher& h) {
-  return h.ids && h.t && h.K > 0 && h.K <= TOP_MAX &&
-         (h.dt == KDT_F32 || h.dt == KDT_BF16 || h.dt == KDT_F16);
+
+template <int DT, int MODE, bool ENT, bool TOP>
+__global__ __launch_bounds__(JOIN_NT) void vocab_join_kernel(const Fwd a, int splits) {
+  constexpr int NT = JOIN_NT;
+  __shared__ float red[NT / 64];
+  const long long row = blockIdx.x;
+  const bool skip = MODE == DISTILL ? !has_teacher<NT>(a, row, red)
+                                    : a.targets && a.targets[row] == a.ignore;
+  if (skip) return;                                // the first kernel wrote the row
+  const Part* p = (const Part*)a.ws + row * splits;
+  float m = -INFINITY, s = 0.f, sum = 0.f;
+  if (threadIdx.x < splits) {
+    const Part v = p[threadIdx.x];
+    m = v.m;
+    s = v.s;
+    sum = v.a;
+  }
+  join<NT, true>(a.inv_t * LOG2E, red, m, s, sum);
+  if constexpr (MODE == DISTILL) {
+    __shared__ SlotShared slots;
+    distill_row<DT, NT>(a, row, m, logf(s), slots, red);
+  } else {
+    float L;
+    logprob_row<DT, NT>(a, row, m, s, sum, L);
+    if constexpr (TOP) {
+      __shared__ uint64_t cand[JOIN_CAND], head[MAX_SPLITS], bound_s;
+      __shared__ int count;
+      const uint64_t* keys =
+          (const uint64_t*)((const Part*)a.ws + a.rows * splits) + row * splits * a.k;
+      const int depth = join_depth(a.k, splits), r = (a.k + depth - 1) / depth;
+      const uint64_t mine = threadIdx.x < splits ? keys[threadIdx.x * a.k + depth - 1] : 0;
+      if (threadIdx.x < MAX_SPLITS) head[threadIdx.x] = mine;
+      if (threadIdx.x == 0) {
+        count = 0;
+        bound_s = 1;
+      }
+      __syncthreads();
+      if (threadIdx.x < splits && mine) {
+        int above = 0;
+        for (int j = 0; j < splits; ++j) above += head[j] > mine;
+        if (above == r - 1) bound_s = mine;        // keys are unique: one thread
+      }
+      __syncthreads();
+      const uint64_t bound = bound_s;
+      for (int i = threadIdx.x; i < splits * a.k; i += NT)
+        if (keys[i] >= bound) {
+          const int c = atomicAdd(&count, 1);
+          if (c < JOIN_CAND) cand[c] = keys[i];
+        }
+      __syncthreads();
+      const int n = count < JOIN_CAND ? count : JOIN_CAND;
+      for (int c = threadIdx.x; c < n; c += NT) {
+        const uint64_t v = cand[c];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += cand[j] > v;
+        if (rank < a.k) {
+          a.top_ids[row * a.k + rank] = (uint32_t)~(uint32_t)v;
+          a.top_lp[row * a.k + rank] = log_prob(key_value((uint32_t)(v >> 32)), m, L, a.inv_t);
+        }
+      }
+    }
+  }
+}
+
+// One workgroup writes BWD_TILES tiles of four 16-byte accesses a thread, then
+// corrects the few elements that carry the target's or the teacher's mass.
+constexpr int BWD_NT = 256, BWD_TILES = 1;
+
+template <int DT> constexpr int bwd_chunk() { return BWD_NT * row_vec<DT>() * 4 * BWD_TILES; }
+
+template <int DT, int MODE, bool ENT>
+__global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int splits) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>(), U = 4, STEP = BWD_NT * V, CHUNK = bwd_chunk<DT>();
+  const long long row = blockIdx.x / splits;
+  const int n = (int)a.V, begin = blockIdx.x % splits * CHUNK;
+  const int end = n - begin < CHUNK ? n : begin + CHUNK;
+  const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ld;
+  AS1 raw_t* dx = gptr((raw_t*)a.dx) + row * a.V;
+  const float M = a.stats[2 * row], L = a.stats[2 * row + 1];
+  const long long tgt = MODE == LOGPROB && a.targets ? a.targets[row] : 0;
+  const bool zero = M == -INFINITY || (MODE == LOGPROB && a.targets && tgt == a.ignore);
+  float g = a.g ? a.g[row * a.gs] : 0.f;
+  if (MODE == LOGPROB && a.g && (tgt < 0 || tgt >= n)) g = NAN;
+  const float gh = ENT ? a.gh[row * a.ghs] : 0.f, H = ENT ? a.entropy[row] : 0.f;
+  const float sign = MODE == LOGPROB ? -a.inv_t : a.inv_t;
+  const float gs = g * sign, ghs = gh * sign;
+  // p_i (g + gh (lp_i + H)), the correction's mass apart
+  auto value = [&](float xi) {
+    const float lp = (xi - M) * a.inv_t - L, p = __builtin_amdgcn_exp2f(lp * LOG2E);
+    return ENT ? p * fmaf(ghs, fmaxf(lp, LOWEST) + H, gs) : p * gs;
+  };
+  for (int at = begin; at < end; at += U * STEP) {
+    const int i = at + threadIdx.x * V;
+    float f[U * V];
+    if (zero) {
+#pragma unroll
+      for (int e = 0; e < U * V; ++e) f[e] = 0.f;
+    } else if (at + U * STEP <= end) {
+      u32x4n raw[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = *(const AS1 u32x4u*)(x + i + u * STEP);
+#pragma unroll
+      for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) fetch<DT>(x, i + u * STEP, end, n, f + u * V);
+    }
+    if (!zero) {
+#pragma unroll
+      for (int e = 0; e < U * V; ++e) f[e] = value(f[e]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) store_vec<DT, true>(dx, i + u * STEP, end, f + u * V);
+  }
+  if (zero || (MODE == LOGPROB && !a.g)) return;
+  __syncthreads();                       // the workgroup's stores come first
+  if (MODE == LOGPROB) {
+    if (threadIdx.x == 0 && tgt >= begin && tgt < end)
+      dx[tgt] = DTypeTraits<DT>::from_f32(value(DTypeTraits<DT>::to_f32(x[tgt])) - gs);
+  } else {
+    for (int j = threadIdx.x; j < a.K; j += BWD_NT) {
+      const int id = a.keep_ids[row * a.K + j];
+      if (id >= begin && id < end)
+        dx[id] = DTypeTraits<DT>::from_f32(
+            gs * (__builtin_amdgcn_exp2f(((DTypeTraits<DT>::to_f32(x[id]) - M) * a.inv_t - L) * LOG2E) -
+                  a.keep_q[row * a.K + j]));
+    }
+  }
+}
+
+// Threads a workgroup: a wave where a row is at most eight 16-byte accesses a
+// lane and its alternatives are fewer than half the lanes.
+int fwd_threads(int dt, long long V, int k) {
+  const int vec = dt == KDT_F32 ? 4 : 8;
+  return V <= 64 * vec * 8 && k <= 32 ? 64 : 256;
+}
+
+// Workgroups a row: enough to have four for every CU, but none with less than
+// two 16-byte accesses a thread.
+int fwd_splits(int dt, long long rows, long long V, int k) {
+  if (fwd_threads(dt, V, k) == 64) return 1;
+  const long long least = 256LL * (dt == KDT_F32 ? 4 : 8) * 2, most = (V + least - 1) / least;
+  long long n = (1024 + rows - 1) / rows;
+  if (n > most) n = most;
+  if (n > MAX_SPLITS) n = MAX_SPLITS;
+  return n < 1 || rows >= 512 ? 1 : (int)n;
+}
+
+bool dtype_ok(int dt) { return dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16; }
+
+template <int DT, int MODE, bool ENT, bool TOP>
+void launch_fwd(const Fwd& a, hipStream_t st) {
+  const int splits = fwd_splits(a.dt, a.rows, a.V, a.k);
+  if (splits == 1 && fwd_threads(a.dt, a.V, a.k) == 64) {
+    hipLaunchKernelGGL((vocab_fwd_kernel<DT, 64, MODE, ENT, TOP>), dim3((unsigned)a.rows),
+                       dim3(64), 0, st, a, 1, (int)a.V);
+    return;
+  }
+  const int vec = row_vec<DT>();
+  const int chunk = (int)((a.V + splits - 1) / splits + vec - 1) / vec * vec;
+  hipLaunchKernelGGL((vocab_fwd_kernel<DT, 256, MODE, ENT, TOP>),
+                     dim3((unsigned)(a.rows * splits)), dim3(256), 0, st, a, splits, chunk);
+  if (splits > 1)
+    hipLaunchKernelGGL((vocab_join_kernel<DT, MODE, ENT, TOP>), dim3((unsigned)a.rows),
+                       dim3(JOIN_NT), 0, st, a, splits);
+}
+
+template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
+  if (a.loss) launch_fwd<DT, DISTILL, false, false>(a, st);
+  else if (a.k && a.entropy) launch_fwd<DT, LOGPROB, true, true>(a, st);
+  else if (a.k) launch_fwd<DT, LOGPROB, false, true>(a, st);
+  else if (a.entropy) launch_fwd<DT, LOGPROB, true, false>(a, st);
+  else launch_fwd<DT, LOGPROB, false, false>(a, st);
+}
+
+template <int DT> void launch_bwd(const Bwd& a, hipStream_t st) {
+  const int splits = (int)((a.V + bwd_chunk<DT>() - 1) / bwd_chunk<DT>());
+  const dim3 grid((unsigned)(a.rows * splits)), block(BWD_NT);
+  if (a.keep_ids)
+    hipLaunchKernelGGL((vocab_bwd_kernel<DT, DISTILL, false>), grid, block, 0, st, a, splits);
+  else if (a.gh)
+    hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, true>), grid, block, 0, st, a, splits);
+  else
+    hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, false>), grid, block, 0, st, a, splits);
 }
 
 }  // namespace
 
-#define VOCAB_LAUNCH(kernel, dt, grid, stream, args)                                          \
-  do {                                                                                        \
-    if (dt == KDT_F32)                                                                        \
-      hipLaunchKernelGGL(kernel<KDT_F32>, grid, dim3(NT), 0, stream, args);                   \
-    else if (dt == KDT_BF16)                                                                  \
-      hipLaunchKernelGGL(kernel<KDT_BF16>, grid, dim3(NT), 0, stream, args);                  \
-    else                                                                                      \
-      hipLaunchKernelGGL(kernel<KDT_F16>, grid, dim3(NT), 0, stream, args);                   \
-  } while (0)
-
 KFAC_API int kfac_vocab_top_max() { return TOP_MAX; }
 
-// targets null: no logprob; entropy null: none; k 0: no alternatives.
-// stats: (M, L) a row, for the backward pass.
-KFAC_API int kfac_logprob_forward(const void* x, long long ld, int dt, long long rows,
-                                  long long V, float inv_t, const long long* targets,
-                                  long long ignore, int k, float* logprob, float* entropy,
-                                  float* top_lp, long long* top_ids, float* stats,
-                                  hipStream_t stream) {
-  LogprobArgs a = {{x, ld, rows, V, inv_t}, targets, ignore, logprob, entropy, top_lp, stats,
-                   top_ids, k};
-  if (!row_ok(a.r, dt) || !stats || k < 0 || k > TOP_MAX || k > V || (logprob && !targets) ||
-      (k && (!top_lp || !top_ids)))
+// bytes of the workspace of one forward call (0: none)
+KFAC_API long long kfac_vocab_ws_bytes(int dt, long long rows, long long V, int k) {
+  const int splits = fwd_splits(dt, rows, V, k);
+  return splits == 1 ? 0 : rows * splits * (long long)(sizeof(Part) + 8LL * k);
+}
+
+// The argument record of ops/vocab.py (`bytes`: its size there).  Log
+// probabilities: targets null: no logprob; entropy null: none; k 0: no
+// alternatives.  Distillation: loss set, with ids, teacher, keep_ids, keep_q.
+KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t stream) {
+  if (bytes != (int)sizeof(Fwd)) return -2;
+  const Fwd a = *args;
+  if (!a.x || a.rows <= 0 || a.V <= 0 || a.V > MAX_V || a.rows > 0x7fffffffLL / MAX_SPLITS ||
+      !(a.inv_t > 0.f) || !dtype_ok(a.dt) || !a.stats)
     return -2;
-  VOCAB_LAUNCH(logprob_fwd_kernel, dt, dim3((unsigned)rows), stream, a);
+  if (a.loss ? !a.ids || !a.teacher || !a.keep_ids || !a.keep_q || !dtype_ok(a.tdt) || a.K < 1 ||
+                   a.K > TOP_MAX || a.k
+             : a.k < 0 || a.k > TOP_MAX || a.k > a.V || (a.logprob && !a.targets) ||
+                   (a.k && (!a.top_lp || !a.top_ids)))
+    return -2;
+  if (!a.ws && kfac_vocab_ws_bytes(a.dt, a.rows, a.V, a.k)) return -2;
+  if (a.dt == KDT_F32) launch_fwd_any<KDT_F32>(a, stream);
+  else if (a.dt == KDT_BF16) launch_fwd_any<KDT_BF16>(a, stream);
+  else launch_fwd_any<KDT_F16>(a, stream);
   return (int)hipGetLastError();
 }
 
-// g, gh: gradients of logprob and entropy, one a row at a distance of gs, ghs
-// elements (0: the same for every row); either may be null
-KFAC_API int kfac_logprob_backward(const void* x, long long ld, int dt, long long rows,
-                                   long long V, float inv_t, const long long* targets,
-                                   long long ignore, const float* stats, const float* entropy,
-                                   const float* g, long long gs, const float* gh, long long ghs,
-                                   void* dx, hipStream_t stream) {
-  LogprobBwd a = {{x, ld, rows, V, inv_t}, targets, ignore, stats, entropy, g, gh, gs, ghs, dx};
-  if (!row_ok(a.r, dt) || !stats || !dx || (g && !targets) || (gh && !entropy)) return -2;
-  VOCAB_LAUNCH(logprob_bwd_kernel, dt, dim3((unsigned)rows), stream, a);
-  return (int)hipGetLastError();
-}
-
-KFAC_API int kfac_distill_forward(const void* x, long long ld, int dt, long long rows,
-                                  long long V, float inv_t, const long long* ids,
-                                  const void* teacher, int tdt, int K, float* loss, float* stats,
-                                  hipStream_t stream) {
-  DistillArgs a = {{x, ld, rows, V, inv_t}, {ids, teacher, tdt, K}, loss, stats};
-  if (!row_ok(a.r, dt) || !teacher_ok(a.h) || !loss || !stats) return -2;
-  VOCAB_LAUNCH(distill_fwd_kernel, dt, dim3((unsigned)rows), stream, a);
-  return (int)hipGetLastError();
-}
-
-KFAC_API int kfac_distill_backward(const void* x, long long ld, int dt, long long rows,
-                                   long long V, float inv_t, const long long* ids,
-                                   const void* teacher, int tdt, int K, const float* stats,
-                                   const float* g, long long gs, void* dx, hipStream_t stream) {
-  DistillBwd a = {{x, ld, rows, V, inv_t}, {ids, teacher, tdt, K}, stats, g, gs, dx};
-  if (!row_ok(a.r, dt) || !teacher_ok(a.h) || !stats || !g || !dx) return -2;
-  VOCAB_LAUNCH(distill_bwd_kernel, dt, dim3((unsigned)rows), stream, a);
+// g, gh: gradients of logprob (or of the loss) and of the entropy, one a row at
+// a distance of gs, ghs elements (0: the same for every row); gh, and g of log
+// probabilities, may be null
+KFAC_API int kfac_vocab_backward(const KfacVocabBwd* args, int bytes, hipStream_t stream) {
+  if (bytes != (int)sizeof(Bwd)) return -2;
+  const Bwd a = *args;
+  if (!a.x || !a.dx || !a.stats || a.rows <= 0 || a.V <= 0 || a.V > MAX_V ||
+      a.rows > 0x7fffffffLL / ((a.V + 4095) / 4096) || !(a.inv_t > 0.f) || !dtype_ok(a.dt))
+    return -2;
+  if (a.keep_ids ? !a.keep_q || !a.g || a.K < 1 || a.K > TOP_MAX
+                 : (!a.g && !a.gh) || (a.g && !a.targets) || (a.gh && !a.entropy))
+    return -2;
+  if (a.dt == KDT_F32) launch_bwd<KDT_F32>(a, stream);
+  else if (a.dt == KDT_BF16) launch_bwd<KDT_BF16>(a, stream);
+  else launch_bwd<KDT_F16>(a, stream);
   return (int)hipGetLastError();
 }

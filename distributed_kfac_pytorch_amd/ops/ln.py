@@ -32,73 +32,82 @@ __all__ = ['layer_norm', 'eligible', 'ENABLED']
 
 ENABLED = os.environ.get('KFAC_FUSED_LN', '1') != '0'
 
-_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # csrc/common.h
 
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _code(t):
-    return 0 if t is None else _lib.DTYPE_CODE[t.dtype]
+# csrc/ln.hip KfacLnFwd, KfacLnBwd
+_fwd = _lib.PackedCall('kfac_ln_forward', '8P4q5if0P')
+_bwd = _lib.PackedCall('kfac_ln_backward', '11P5q6i0P')
 
 
 def eligible(x, normalized_shape, weight=None, bias=None, z=None):
     """True where the kernels run (see the module's text)."""
-    if not (ENABLED and x.is_cuda and x.dtype in _TYPES and x.numel() > 0):
+    if not (ENABLED and x.is_cuda and x.dtype in _CODE and x.numel() > 0):
         return False
     n = len(normalized_shape)
-    if n == 0 or tuple(x.shape[-n:]) != normalized_shape:
+    if n == 0 or x.shape[-n:] != normalized_shape:
         return False
-    if z is not None and (z.shape != x.shape or z.dtype not in _TYPES or z.device != x.device):
+    if z is not None and (z.shape != x.shape or z.dtype not in _CODE or z.device != x.device):
         return False
     for p in (weight, bias):
-        if p is not None and (p.dtype not in _TYPES or p.device != x.device or
-                              tuple(p.shape) != normalized_shape):
+        if p is not None and (p.dtype not in _CODE or p.device != x.device or
+                              p.shape != normalized_shape):
             return False
     return _lib.plain_tensors(x, z, weight, bias)
 
 
 def _rows(t, rows, D):
-    """t as (rows, D) with contiguous rows (a copy where no view has them) and
-    the distance between rows."""
-    if t.is_contiguous():
-        return t, D
-    t = t.reshape(rows, D)
-    if D > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0)
+    """(t as (rows, D) with contiguous rows -- a copy where no view has them --,
+    its address, the distance between rows, its type's code); zeros for None."""
+    if t is None:
+        return None, 0, 0, 0
+    ld = D
+    if not t.is_contiguous():
+        t = t.reshape(rows, D)
+        if D > 1 and t.stride(1) != 1:
+            t = t.contiguous()
+        ld = t.stride(0)
+    return t, t.data_ptr(), ld, _CODE[t.dtype]
 
 
-def _forward(x, z, weight, bias, D, eps, ydtype):
-    """(y, s, mean, rstd); s is x without z."""
-    L = _lib.lib()
+def _vector(p):
+    """(weight or bias contiguous, its address, its type's code); zeros for None."""
+    if p is None:
+        return None, 0, 0
+    p = p.contiguous()
+    return p, p.data_ptr(), _CODE[p.dtype]
+
+
+def _forward(x, z, weight, bias, D, eps, ydtype, keep):
+    """(y, s, mean and rstd where `keep`); s is x without z."""
     rows = x.numel() // D
     if z is not None and x.dtype != z.dtype and x.dtype != torch.float32:
         x, z = z, x                              # the sum's type is the wider one's: fp32 ...
         if x.dtype != torch.float32:
             x = x.float()                        # ... also for bf16 + fp16
-    y = torch.empty(x.shape, dtype=x.dtype if ydtype is None else ydtype, device=x.device)
-    s = None if z is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    xr, ldx = _rows(x, rows, D)
-    zr, ldz = (None, 0) if z is None else _rows(z, rows, D)
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.contiguous()
-    with _lib.device_guard(x.device):
-        _lib.check(L.kfac_ln_forward(
-            xr.data_ptr(), ldx, _code(x), _ptr(zr), ldz, _code(z), _ptr(w), _code(w), _ptr(b),
-            _code(b), y.data_ptr(), _code(y), _ptr(s), stats.data_ptr(),
-            stats.data_ptr() + 4 * rows, rows, D, float(eps), _lib.stream(x.device)),
-            'kfac_ln_forward')
-    return y, (x if z is None else s), stats
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    y = torch.empty(shape, dtype=ydtype or dtype, device=dev)
+    s, sp = x, 0
+    if z is not None:
+        s = torch.empty(shape, dtype=dtype, device=dev)
+        sp = s.data_ptr()
+    stats, mp = None, 0
+    if keep:
+        stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+        mp = stats.data_ptr()
+    x, xp, ldx, code = _rows(x, rows, D)
+    z, zp, ldz, zcode = _rows(z, rows, D)
+    w, wp, wcode = _vector(weight)
+    b, bp, bcode = _vector(bias)
+    _fwd(dev, xp, zp, wp, bp, y.data_ptr(), sp, mp, mp and mp + 4 * rows, ldx, ldz, rows, D,
+         code, zcode, wcode, bcode, _CODE[y.dtype], eps)
+    return y, s, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, z, weight, bias, shape, eps, ydtype):
-        y, s, stats = _forward(x, z, weight, bias, math.prod(shape), eps, ydtype)
-        ctx.save_for_backward(s, weight, bias, stats)
+        y, s, ctx.stats = _forward(x, z, weight, bias, math.prod(shape), eps, ydtype, True)
+        ctx.save_for_backward(s, weight, bias)
         ctx.shape, ctx.eps = shape, eps
         ctx.xdtype, ctx.zdtype = x.dtype, None if z is None else z.dtype
         ctx.set_materialize_grads(False)
@@ -106,54 +115,62 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, ds=None):
-        s, weight, bias, stats = ctx.saved_tensors
         if dy is None and ds is None:
             return (None,) * 7
+        s, weight, bias = ctx.saved_tensors
+        dw = db = dl = None
         if dy is None:
-            d, dw, db = ds, None, None
+            d = ds
         elif torch.is_grad_enabled():            # create_graph: differentiable operations
             d, dw, db = _differentiable(ctx, s, weight, bias, dy, ds)
         else:
-            d, dw, db = _backward(ctx, s, weight, bias, stats, dy, ds)
-        if type(d) is tuple:
-            dx, dz = d
-        else:
-            dx = None if d is None else d.to(ctx.xdtype)
-            dz = None if d is None or ctx.zdtype is None else d.to(ctx.zdtype)
-        return dx, dz, dw, db, None, None, None
+            d, dl, dw, db = _backward(ctx, s, weight, bias, dy, ds)
+
+        def of(dtype):
+            if d is None or dtype is None:
+                return None
+            return d if dtype == d.dtype else dl if dl is not None and dtype == dl.dtype \
+                else d.to(dtype)
+        need = ctx.needs_input_grad
+        return (of(ctx.xdtype) if need[0] else None, of(ctx.zdtype) if need[1] else None, dw, db,
+                None, None, None)
 
 
-def _backward(ctx, s, weight, bias, stats, dy, ds):
-    """((dx, dz), dw, db), each None where it is not asked for."""
-    L = _lib.lib()
+def _backward(ctx, s, weight, bias, dy, ds):
+    """(gradient of s, the same in the type of whichever of x and z is narrower,
+    dw, db), each None where it is not asked for."""
     D = math.prod(ctx.shape)
     rows = s.numel() // D
+    dev, dtype, shape = s.device, s.dtype, s.shape
     need_x, need_z, need_w, need_b = ctx.needs_input_grad[:4]
-    sr, lds = _rows(s, rows, D)
-    gr, ldg = _rows(dy, rows, D)
-    er, lde = (None, 0) if ds is None else _rows(ds, rows, D)
-    dx = torch.empty(s.shape, dtype=s.dtype, device=s.device) if need_x or need_z else None
-    # one of x and z may be narrower than their sum: its gradient is stored on its own
-    low = next((t for t in (ctx.xdtype, ctx.zdtype) if t not in (None, s.dtype)), None)
-    same = dx is None or low is None or ctx.xdtype == ctx.zdtype
-    dl = None if same else torch.empty(s.shape, dtype=low, device=s.device)
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=s.device) if need_w else None
-    db = torch.empty(bias.shape, dtype=bias.dtype, device=s.device) if need_b else None
-    part = torch.empty(L.kfac_ln_ws_floats(_code(s), rows, D), dtype=torch.float32, device=s.device) \
-        if need_w or need_b else None
-    w = None if weight is None else weight.contiguous()
-    with _lib.device_guard(s.device):
-        _lib.check(L.kfac_ln_backward(
-            gr.data_ptr(), ldg, _code(gr), _ptr(er), lde, sr.data_ptr(), lds, _code(s), _ptr(w),
-            _code(w), _code(bias), stats.data_ptr(), stats.data_ptr() + 4 * rows, _ptr(dx),
-            _ptr(dl), _code(dl), _ptr(dw), _ptr(db), _ptr(part), rows, D,
-            _lib.stream(s.device)), 'kfac_ln_backward')
-
-    def of(dtype):
-        if dx is None or dtype is None:
-            return None
-        return dx if dtype == s.dtype else dl if dl is not None and dtype == low else dx.to(dtype)
-    return (of(ctx.xdtype) if need_x else None, of(ctx.zdtype) if need_z else None), dw, db
+    d = dl = dw = db = part = None
+    dp = lp = wgp = bgp = pp = lcode = 0
+    if need_x or need_z:
+        d = torch.empty(shape, dtype=dtype, device=dev)
+        dp = d.data_ptr()
+        low = ctx.xdtype if ctx.xdtype != dtype else ctx.zdtype
+        if low is not None and low != dtype:
+            dl = torch.empty(shape, dtype=low, device=dev)
+            lp, lcode = dl.data_ptr(), _CODE[low]
+    w, wp, wcode = _vector(weight)
+    if need_w:
+        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+        wgp = dw.data_ptr()
+    if need_b:
+        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+        bgp = db.data_ptr()
+    code = _CODE[dtype]
+    if need_w or need_b:
+        part = torch.empty(_lib.lib().kfac_ln_ws_floats(code, rows, D), dtype=torch.float32,
+                           device=dev)
+        pp = part.data_ptr()
+    s, sp, lds, _ = _rows(s, rows, D)
+    g, gp, ldg, gcode = _rows(dy, rows, D)
+    e, ep, lde, _ = _rows(ds, rows, D)
+    mp = ctx.stats.data_ptr()
+    _bwd(dev, gp, ep, sp, wp, mp, mp + 4 * rows, dp, lp, wgp, bgp, pp, ldg, lde, lds, rows, D,
+         code, lcode, wcode, 0 if bias is None else _CODE[bias.dtype], gcode, 0)
+    return d, dl, dw, db
 
 
 def _differentiable(ctx, s, weight, bias, dy, ds):
@@ -182,5 +199,5 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, z=None):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (x, z, weight, bias)):
         return _LayerNorm.apply(x, z, weight, bias, shape, eps, ydtype)
-    y, s, _ = _forward(x, z, weight, bias, math.prod(shape), eps, ydtype)
+    y, s, _ = _forward(x, z, weight, bias, math.prod(shape), eps, ydtype, False)
     return y if z is None else (y, s)

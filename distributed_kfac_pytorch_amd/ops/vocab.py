@@ -30,7 +30,12 @@ __all__ = ['token_logprobs', 'topk_distill_loss', 'TokenLogprobs', 'TOP_MAX']
 # most alternatives a row, and most slots of a teacher's row (csrc/vocab.hip)
 TOP_MAX = 128
 
-_GPU_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # csrc/common.h
+_GPU_TYPES = tuple(_CODE)
+
+# csrc/vocab.hip KfacVocabFwd, KfacVocabBwd
+_fwd = _lib.PackedCall('kfac_vocab_forward', '13P4q4if0P')
+_bwd = _lib.PackedCall('kfac_vocab_backward', '9P6q2if0P')
 
 
 class TokenLogprobs(NamedTuple):
@@ -50,12 +55,14 @@ def _check(name, logits, temperature):
     if logits.is_cuda and logits.dtype not in _GPU_TYPES:
         raise TypeError('{}: GPU logits must be fp32, bf16 or fp16, got {}'.format(
             name, logits.dtype))
-    if logits.shape[-1] > 2 ** 31 - 1 or logits.numel() // logits.shape[-1] > 2 ** 31 - 1:
-        raise ValueError('{}: more than 2^31 - 1 rows or columns'.format(name))
+    V = logits.shape[-1]
+    rows = logits.numel() // V
+    if V > 2 ** 30 or rows >= 2 ** 25 or rows * -(-V // 4096) >= 2 ** 31:
+        raise ValueError('{}: logits of shape {} are too many rows or columns'.format(
+            name, tuple(logits.shape)))
     temperature = float(temperature)
-    # 1 / T has to be an ordinary fp32 number
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError('{}: temperature must be in [1e-30, 1e30], got {}'.format(
+    if not 1e-4 <= temperature <= 1e4:
+        raise ValueError('{}: temperature must be in [1e-4, 1e4], got {}'.format(
             name, temperature))
     return 1.0 / temperature
 
@@ -77,30 +84,40 @@ def _check_plain(name, *tensors):
                         'levels and compile traces'.format(name))
 
 
-def _rows(t):
-    """(t as (rows, V) with contiguous rows, distance between rows)."""
-    V = t.shape[-1]
+def _rows(t, rows, V):
+    """(t as (rows, V) with contiguous rows, the distance between rows)."""
     if t.is_contiguous():
         return t, V
-    t = t.reshape(-1, V)
+    t = t.reshape(rows, V)
     if V > 1 and t.stride(1) != 1:
         t = t.contiguous()
     return t, t.stride(0)
 
 
-def _row_grad(g, rows):
-    """(g or a copy of it, distance between its rows): the gradient of a mean or
-    sum is one number expanded (distance 0)."""
+def _row_grad(g):
+    """(g or a copy of it, its address, the distance between its rows): the
+    gradient of a mean or sum is one number expanded (distance 0)."""
     if g is None:
+        return None, 0, 0
+    if g.is_contiguous():
+        return g, g.data_ptr(), 1
+    if not any(g.stride()):
+        return g, g.data_ptr(), 0
+    g = g.contiguous()
+    return g, g.data_ptr(), 1
+
+
+def _workspace(code, rows, V, k, dev):
+    """(workspace or None, its address) of one forward call."""
+    n = _lib.lib().kfac_vocab_ws_bytes(code, rows, V, k)
+    if not n:
         return None, 0
-    g = g.to(torch.float32)
-    if all(s == 0 or n == 1 for s, n in zip(g.stride(), g.shape)):
-        return g, 0
-    return g.contiguous(), 1
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    return ws, ws.data_ptr()
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 # -------------------------------------------------------- CPU: the formulas
@@ -144,19 +161,18 @@ class _TokenLogprobs(torch.autograd.Function):
         h = out() if entropy else None
         tl, ti = (out(k), out(k, dtype=torch.int64)) if k else (None, None)
         tgt = None if targets is None else targets.to(torch.int64).contiguous()
+        stats = None
         if rows == 0:
-            stats = None
+            pass
         elif _lib.use_native(logits):
-            x, ld = _rows(logits)
-            stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
-            with _lib.device_guard(dev):
-                _lib.check(_lib.lib().kfac_logprob_forward(
-                    x.data_ptr(), ld, _lib.DTYPE_CODE[x.dtype], rows, V, inv_t, _ptr(tgt), ignore,
-                    k, _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti), stats.data_ptr(),
-                    _lib.stream(dev)), 'kfac_logprob_forward')
+            x, ld = _rows(logits, rows, V)
+            code = _CODE[x.dtype]
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+            ws, wp = _workspace(code, rows, V, k, dev)
+            _fwd(dev, x.data_ptr(), _ptr(tgt), _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti),
+                 stats.data_ptr(), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, inv_t)
         else:
             x, M, L, all_lp = _cpu_stats(logits.reshape(rows, V), inv_t)
-            stats = torch.stack([M, L], 1)
             skip = torch.zeros(rows, dtype=torch.bool) if tgt is None else \
                 tgt.reshape(-1) == ignore
             if lp is not None:
@@ -173,13 +189,14 @@ class _TokenLogprobs(torch.autograd.Function):
                          .view(shape + (k,)))
         if k:
             ctx.mark_non_differentiable(tl, ti)
-        ctx.save_for_backward(logits, tgt, stats, h)
+        ctx.save_for_backward(logits, tgt, h)
+        ctx.stats = stats
         return lp, h, tl, ti
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, gh, _tl, _ti):
-        logits, tgt, stats, h = ctx.saved_tensors
+        logits, tgt, h = ctx.saved_tensors
         if g is None and gh is None:
             return (None,) * 6
         V = logits.shape[-1]
@@ -188,13 +205,10 @@ class _TokenLogprobs(torch.autograd.Function):
         if rows == 0:
             return dx, None, None, None, None, None
         if _lib.use_native(logits):
-            x, ld = _rows(logits)
-            (g, gs), (gh, ghs) = _row_grad(g, rows), _row_grad(gh, rows)
-            with _lib.device_guard(logits.device):
-                _lib.check(_lib.lib().kfac_logprob_backward(
-                    x.data_ptr(), ld, _lib.DTYPE_CODE[x.dtype], rows, V, ctx.inv_t, _ptr(tgt),
-                    ctx.ignore, stats.data_ptr(), _ptr(h), _ptr(g), gs, _ptr(gh), ghs,
-                    dx.data_ptr(), _lib.stream(logits.device)), 'kfac_logprob_backward')
+            x, ld = _rows(logits, rows, V)
+            (g, gp, gs), (gh, ghp, ghs) = _row_grad(g), _row_grad(gh)
+            _bwd(logits.device, x.data_ptr(), ctx.stats.data_ptr(), _ptr(h), _ptr(tgt), gp, ghp, 0,
+                 0, dx.data_ptr(), ld, rows, V, ctx.ignore, gs, ghs, _CODE[x.dtype], 0, ctx.inv_t)
         else:
             _, M, _, lp = _cpu_stats(logits.reshape(rows, V), ctx.inv_t)
             p = lp.exp()
@@ -271,41 +285,43 @@ class _TopkDistill(torch.autograd.Function):
         teacher = teacher.contiguous()
         K = ids.shape[-1]
         loss = torch.empty(logits.shape[:-1], dtype=dt, device=dev)
-        stats = None
+        ctx.kept = None
         if rows and _lib.use_native(logits):
-            x, ld = _rows(logits)
-            stats = torch.empty(rows, 2, dtype=torch.float32, device=dev)
-            with _lib.device_guard(dev):
-                _lib.check(_lib.lib().kfac_distill_forward(
-                    x.data_ptr(), ld, _lib.DTYPE_CODE[x.dtype], rows, V, inv_t, ids.data_ptr(),
-                    teacher.data_ptr(), _lib.DTYPE_CODE[teacher.dtype], K, loss.data_ptr(),
-                    stats.data_ptr(), _lib.stream(dev)), 'kfac_distill_forward')
+            x, ld = _rows(logits, rows, V)
+            code = _CODE[x.dtype]
+            # for the backward pass: (M, L) of the rows, each id once and its mass
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+            at = torch.empty(rows * K, dtype=torch.int32, device=dev)
+            mass = torch.empty(rows * K, dtype=torch.float32, device=dev)
+            ctx.kept = stats, at, mass
+            ws, wp = _workspace(code, rows, V, 0, dev)
+            _fwd(dev, x.data_ptr(), 0, 0, 0, 0, 0, stats.data_ptr(), ids.data_ptr(),
+                 teacher.data_ptr(), loss.data_ptr(), at.data_ptr(), mass.data_ptr(), wp, ld, rows,
+                 V, 0, code, 0, K, _CODE[teacher.dtype], inv_t)
         elif rows:
             lp = _cpu_stats(logits.reshape(rows, V), inv_t)[3]
             some, at, q, logq = _cpu_teacher(ids.reshape(rows, K), teacher.reshape(rows, K), V,
                                              inv_t, dt)
             each = torch.where(q == 0, 0.0, q * (logq - lp.gather(1, at)))
             loss.copy_(torch.where(some, each.sum(1), 0.0).view(loss.shape))
-        ctx.save_for_backward(logits, ids, teacher, stats)
+        ctx.save_for_backward(logits, ids, teacher)
         ctx.inv_t = inv_t
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, ids, teacher, stats = ctx.saved_tensors
+        logits, ids, teacher = ctx.saved_tensors
         V, K = logits.shape[-1], ids.shape[-1]
         rows = logits.numel() // V
         dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if rows and _lib.use_native(logits):
-            x, ld = _rows(logits)
-            g, gs = _row_grad(g, rows)
-            with _lib.device_guard(logits.device):
-                _lib.check(_lib.lib().kfac_distill_backward(
-                    x.data_ptr(), ld, _lib.DTYPE_CODE[x.dtype], rows, V, ctx.inv_t,
-                    ids.data_ptr(), teacher.data_ptr(), _lib.DTYPE_CODE[teacher.dtype], K,
-                    stats.data_ptr(), g.data_ptr(), gs, dx.data_ptr(),
-                    _lib.stream(logits.device)), 'kfac_distill_backward')
+            x, ld = _rows(logits, rows, V)
+            g, gp, gs = _row_grad(g)
+            stats, at, mass = ctx.kept
+            _bwd(logits.device, x.data_ptr(), stats.data_ptr(), 0, 0, gp, 0, at.data_ptr(),
+                 mass.data_ptr(), dx.data_ptr(), ld, rows, V, 0, gs, 0, _CODE[x.dtype], K,
+                 ctx.inv_t)
         elif rows:
             _, M, _, lp = _cpu_stats(logits.reshape(rows, V), ctx.inv_t)
             some, at, q, _ = _cpu_teacher(ids.reshape(rows, K), teacher.reshape(rows, K), V,

@@ -241,7 +241,7 @@ def test_rows_that_are_skipped_are_not_read():
     assert not torch.autograd.grad(loss.sum(), x)[0][1].any()
 
 
-@pytest.mark.parametrize('T', [1e-30, 1e-3, 50.0, 1e30])
+@pytest.mark.parametrize('T', [1e-4, 1e-2, 50.0, 1e4])
 def test_temperatures(T):
     x = logits(4, 777, F32)
     t = x.argmax(1)
@@ -250,9 +250,8 @@ def test_temperatures(T):
     oracle.check('logprobs', r.logprobs, o['logprobs'])
     oracle.check('entropy', r.entropy, o['entropy'])
     oracle.check('top_logprobs', r.top_logprobs, o['top_logprobs'])
-    if T > 1e-10:
-        ids, q = teacher(4, 777, 5, F32)
-        check_distill(x, ids, q, T)
+    ids, q = teacher(4, 777, 5, F32)
+    check_distill(x, ids, q, T)
 
 
 def test_cpu_and_gpu_agree():

@@ -151,6 +151,11 @@ def test_alternatives_have_no_gradient():
     (lambda x, t: vocab.token_logprobs(x), ValueError),
     (lambda x, t: vocab.token_logprobs(x, t, temperature=0.0), ValueError),
     (lambda x, t: vocab.token_logprobs(x, t, temperature=-1.0), ValueError),
+    (lambda x, t: vocab.token_logprobs(x, t, temperature=9e-5), ValueError),
+    (lambda x, t: vocab.token_logprobs(x, t, temperature=2e4), ValueError),
+    (lambda x, t: vocab.token_logprobs(x[:1, :1].expand(2, 2 ** 30 + 1), t), ValueError),
+    (lambda x, t: vocab.token_logprobs(x[:1].expand(2 ** 25, 5), t[:1].expand(2 ** 25)),
+     ValueError),
     (lambda x, t: vocab.token_logprobs(x, t, temperature=math.nan), ValueError),
     (lambda x, t: vocab.token_logprobs(x, t, temperature=math.inf), ValueError),
     (lambda x, t: vocab.topk_distill_loss(x, t, x), ValueError),

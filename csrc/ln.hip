@@ -168,28 +168,65 @@ template <int TR> struct RowSum {      // sums over the TR threads of a row
   }
 };
 
-// z's or dy's E elements in another type than the stream's (uniform over the launch)
+// E elements in one of the three types (uniform over the launch): the weights,
+// and z, dy, dz or y where their type is not the stream's.  V elements in
+// accesses of at most 16 bytes; the access past the row's end one by one.
+template <int DT, int V, int R>
+__device__ __forceinline__ void load_as(const void* p, long long off, int t0, int step, int n,
+                                        float* f) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  typedef raw_t vec_t __attribute__((ext_vector_type(V)));
+  typedef vec_t vec_u __attribute__((aligned(sizeof(raw_t))));
+  const AS1 raw_t* q = gptr((const raw_t*)p) + off;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = t0 + r * step;
+    if (i + V <= n) {
+      const vec_t v = *(const AS1 vec_u*)(q + i);
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[r * V + e] = DTypeTraits<DT>::to_f32(v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        f[r * V + e] = i + e < n ? DTypeTraits<DT>::to_f32(q[i + e]) : 0.f;
+    }
+  }
+}
+template <int DT, int V, int R>
+__device__ __forceinline__ void store_as(void* p, long long off, int t0, int step, int n,
+                                         const float* f) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  typedef raw_t vec_t __attribute__((ext_vector_type(V)));
+  typedef vec_t vec_u __attribute__((aligned(sizeof(raw_t))));
+  AS1 raw_t* q = gptr((raw_t*)p) + off;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = t0 + r * step;
+    vec_t v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = DTypeTraits<DT>::from_f32(f[r * V + e]);
+    if (i + V <= n) {
+      *(AS1 vec_u*)(q + i) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i + e < n) q[i + e] = v[e];
+    }
+  }
+}
 template <int V, int R>
 __device__ __forceinline__ void load_other(const void* p, long long off, int dt, int t0, int step,
                                            int n, float* f) {
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int i = t0 + r * step + e;
-      f[r * V + e] = i < n ? ld_any(p, off + i, dt) : 0.f;
-    }
+  if (dt == KDT_F32) load_as<KDT_F32, V, R>(p, off, t0, step, n, f);
+  else if (dt == KDT_BF16) load_as<KDT_BF16, V, R>(p, off, t0, step, n, f);
+  else load_as<KDT_F16, V, R>(p, off, t0, step, n, f);
 }
 template <int V, int R>
 __device__ __forceinline__ void store_other(void* p, long long off, int dt, int t0, int step,
                                             int n, const float* f) {
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int i = t0 + r * step + e;
-      if (i < n) st_any(p, off + i, dt, f[r * V + e]);
-    }
+  if (dt == KDT_F32) store_as<KDT_F32, V, R>(p, off, t0, step, n, f);
+  else if (dt == KDT_BF16) store_as<KDT_BF16, V, R>(p, off, t0, step, n, f);
+  else store_as<KDT_F16, V, R>(p, off, t0, step, n, f);
 }
 
 template <int DT, int TR, int E, bool TAIL>

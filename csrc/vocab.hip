@@ -14,7 +14,7 @@
 // every finite row finite.
 //
 // Forward: ONE pass over the row.  A thread keeps the running maximum m of its
-// elements, s = sum exp((x - m) / T) and a = sum exp((x - m) / T) (x - m), each
+// elements, s = sum exp((x - m) / T) and a = sum exp((x - m) / T) (x - m) / T, each
 // brought to a new maximum once per tile of four 16-byte loads; the threads'
 // (m, s, a) are joined at the end.  The alternatives need no second pass: the
 // k-th largest of the threads' maxima is a bound that at least k elements
@@ -70,9 +70,8 @@ typedef KfacVocabBwd Bwd;
 constexpr int TOP_MAX = 128;      // alternatives, and slots of a teacher's row
 constexpr int MAX_V = 1 << 30;    // elements of a row: 32-bit offsets within it
 constexpr int MAX_SPLITS = 64;    // workgroups a row
-constexpr float LOG2E = 1.4426950408889634f;
-// A distance to the maximum below which exp(d / T) is 0 for every T <= 1e4 that
-// the operators take; a product 0 d stays 0 when d is no lower than this.
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// An exponent far below what exp2 gives 0 for, whose product with that 0 is 0.
 constexpr float LOWEST = -1e9f;
 
 enum Mode { LOGPROB = 0, DISTILL = 1 };
@@ -143,23 +142,51 @@ __device__ __forceinline__ void fetch(const AS1 typename DTypeTraits<DT>::raw_t*
     if (i + e >= end) f[e] = -INFINITY;
 }
 
-// The running (m, s, a) of one thread over a tile of N elements.
+// The running (m, s, a) of one thread over a tile of N elements: s = sum e^(..),
+// a = sum e^(..) u with u = (x - m) / T in units of log 2.  c1 = log2 e / T.
+template <int N, bool ENT>
+__device__ __forceinline__ void fold_any(const float* f, float top, float c1, float& s, float& a) {
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float u = (f[e] - base) * c1, x = __builtin_amdgcn_exp2f(u);
+    s += x;
+    if (ENT) a = fmaf(x, fmaxf(u, LOWEST), a);        // exp(-inf) = 0 times a finite number
+  }
+}
+
+// The same with one instruction less an element, u' = x c1 - R with R = m c1
+// rounded: every u' of the tile is off by the same d = m c1 - R, which is known
+// exactly and taken out of the sums.  Not where R is so large that d is no
+// small number (or no number), and not where an entropy's product meets a -inf.
 template <int N, bool ENT>
 __device__ __forceinline__ void fold(const float* f, float c1, float& m, float& s, float& a) {
   float top = m;
 #pragma unroll
   for (int e = 0; e < N; ++e) top = fmaxf(top, f[e]);
-  const float base = top == -INFINITY ? 0.f : top;
-  const float back = fmaxf(m - base, LOWEST), scale = __builtin_amdgcn_exp2f(back * c1);
+  // the running sums brought to the new maximum
+  const float back = fmaxf((m - (top == -INFINITY ? 0.f : top)) * c1, LOWEST);
+  const float scale = __builtin_amdgcn_exp2f(back);
   if (ENT) a = scale * fmaf(back, s, a);
   s *= scale;
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float d = f[e] - base, x = __builtin_amdgcn_exp2f(d * c1);
-    s += x;
-    if (ENT) a = fmaf(x, fmaxf(d, LOWEST), a);      // exp(-inf) = 0 times a finite number
-  }
   m = top;
+  const float R = top * c1;
+  float st = 0.f, at = 0.f;
+  if (!__any(!(fabsf(R) < 0x1p20f))) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float u = fmaf(f[e], c1, -R), x = __builtin_amdgcn_exp2f(u);
+      st += x;
+      if (ENT) at = fmaf(x, u, at);
+    }
+    if (!ENT || !__any(at != at)) {
+      const float d = fmaf(top, c1, -R), fix = __builtin_amdgcn_exp2f(-d);
+      s = fmaf(st, fix, s);
+      if (ENT) a = fmaf(fmaf(-d, st, at), fix, a);
+      return;
+    }
+  }
+  fold_any<N, ENT>(f, top, c1, s, a);
 }
 
 template <int DT, int NT, bool ENT>
@@ -174,7 +201,8 @@ __device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* 
     u32x4n raw[U];
     float f[U * V];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = *(const AS1 u32x4u*)(x + i + u * STEP);
+    for (int u = 0; u < U; ++u)
+      raw[u] = __builtin_nontemporal_load((const AS1 u32x4u*)(x + i + u * STEP));
 #pragma unroll
     for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
     fold<U * V, ENT>(f, c1, m, s, a);
@@ -191,8 +219,9 @@ __device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* 
 // (m, s, a) joined over the workgroup
 template <int NT, bool ENT>
 __device__ __forceinline__ void join(float c1, float* red, float& m, float& s, float& a) {
-  const float M = Group<NT>::max(m, red), base = M == -INFINITY ? 0.f : M;
-  const float back = fmaxf(m - base, LOWEST), scale = __builtin_amdgcn_exp2f(back * c1);
+  const float M = Group<NT>::max(m, red);
+  const float back = fmaxf((m - (M == -INFINITY ? 0.f : M)) * c1, LOWEST);
+  const float scale = __builtin_amdgcn_exp2f(back);
   if (ENT) a = Group<NT>::sum(scale * fmaf(back, s, a), red);
   s = Group<NT>::sum(s * scale, red);
   m = M;
@@ -454,7 +483,7 @@ __device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M
     a.logprob[row] =
         t < 0 || t >= a.V ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[t]), M, L, a.inv_t);
   }
-  if (a.entropy) a.entropy[row] = M == -INFINITY ? 0.f : L - sum / s * a.inv_t;
+  if (a.entropy) a.entropy[row] = M == -INFINITY ? 0.f : L - sum / s * LN2;
   a.stats[2 * row] = M;
   a.stats[2 * row + 1] = L;
 }

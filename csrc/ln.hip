@@ -38,7 +38,7 @@ namespace {
 typedef KfacLnFwd Fwd;
 typedef KfacLnBwd Bwd;
 
-constexpr int NT = 256;
+constexpr int NT = 256, LT = 1024;     // threads: columns' sums, long rows
 
 __device__ __forceinline__ float ld_any(const void* p, long long i, int dt) {
   if (dt == KDT_F32) return ((const float*)p)[i];
@@ -57,38 +57,99 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   float r = red[0];
-  for (int i = 1; i < NT / 64; ++i) r += red[i];
+  for (int i = 1; i < LT / 64; ++i) r += red[i];
   return r;
 }
 
-__global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const Fwd a) {
-  __shared__ float red[NT / 64];
-  const long long row = blockIdx.x, D = a.D;
-  const long long xo = row * a.ldx, zo = row * a.ldz, yo = row * D;
-  float acc = 0.f;
-  for (long long i = threadIdx.x; i < D; i += NT) {
-    float v = ld_any(a.x, xo + i, a.sdt);
-    if (a.z) {
-      v += ld_any(a.z, zo + i, a.zdt);
-      st_any(a.s, yo + i, a.sdt, v);
-      v = ld_any(a.s, yo + i, a.sdt);    // this thread's own store: the rounded sum is normed
-    }
-    acc += v;
+// Rows that no workgroup's registers hold (and rows shorter than one access):
+// the workgroup walks the row, once for each statistic and once for the
+// result; from the second time on it comes from a cache.
+
+// V elements at i, zeros from n on
+template <int DT>
+__device__ __forceinline__ void walk_load(const AS1 typename DTypeTraits<DT>::raw_t* row,
+                                          long long i, long long n, float* f) {
+  constexpr int V = row_vec<DT>();
+  if (i + V <= n) {
+    vec_to_f32<DT>(*(const AS1 u32x4u*)(row + i), f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = i + e < n ? DTypeTraits<DT>::to_f32(row[i + e]) : 0.f;
   }
-  const void* sp = a.z ? a.s : a.x;
-  const long long so = a.z ? yo : xo;
+}
+// V elements at i of a row of any type (uniform over the launch)
+template <int V>
+__device__ __forceinline__ void walk_any(const void* p, long long off, int dt, long long i,
+                                         long long n, float* f) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) f[e] = i + e < n ? ld_any(p, off + i + e, dt) : 0.f;
+}
+template <int DT>
+__device__ __forceinline__ void walk_other(const void* p, long long off, int dt, long long i,
+                                           long long n, float* f) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  if (dt == DT) walk_load<DT>(gptr((const raw_t*)p) + off, i, n, f);
+  else walk_any<row_vec<DT>()>(p, off, dt, i, n, f);
+}
+template <int DT>
+__device__ __forceinline__ void walk_store(void* p, long long off, int dt, long long i,
+                                           long long n, const float* f) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>();
+  if (dt == DT && i + V <= n) {
+    *(AS1 u32x4u*)(gptr((raw_t*)p) + off + i) = f32_to_vec<DT>(f);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (i + e < n) st_any(p, off + i + e, dt, f[e]);
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(LT) void ln_fwd_long_kernel(const Fwd a) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>(), STEP = LT * V;
+  __shared__ float red[LT / 64];
+  const long long row = blockIdx.x, D = a.D, t0 = threadIdx.x * V;
+  const long long yo = row * D;
+  const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
+  float acc = 0.f;
+  for (long long i = t0; i < D; i += STEP) {
+    float f[V];
+    walk_load<DT>(x, i, D, f);
+    if (a.z) {
+      float g[V];
+      walk_other<DT>(a.z, row * a.ldz, a.zdt, i, D, g);
+#pragma unroll
+      for (int e = 0; e < V; ++e)      // the sum as it is stored is what is normed
+        f[e] = DTypeTraits<DT>::to_f32(DTypeTraits<DT>::from_f32(f[e] + g[e]));
+      walk_store<DT>(a.s, yo, DT, i, D, f);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc += f[e];
+  }
+  const AS1 raw_t* s = a.z ? gptr((const raw_t*)a.s) + yo : x;     // each thread's own stores
   const float mu = block_sum(acc, red) / (float)D;
   acc = 0.f;
-  for (long long i = threadIdx.x; i < D; i += NT) {
-    const float d = ld_any(sp, so + i, a.sdt) - mu;
-    acc = fmaf(d, d, acc);
+  for (long long i = t0; i < D; i += STEP) {
+    float f[V];
+    walk_load<DT>(s, i, D, f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = f[e] - mu;
+      acc = fmaf(d, i + e < D ? d : 0.f, acc);
+    }
   }
   const float rstd = 1.f / sqrtf(block_sum(acc, red) / (float)D + a.eps);
-  for (long long i = threadIdx.x; i < D; i += NT) {
-    float v = (ld_any(sp, so + i, a.sdt) - mu) * rstd;
-    if (a.w) v *= ld_any(a.w, i, a.wdt);
-    if (a.b) v += ld_any(a.b, i, a.bdt);
-    st_any(a.y, yo + i, a.ydt, v);
+  for (long long i = t0; i < D; i += STEP) {
+    float f[V], w[V], b[V];
+    walk_load<DT>(s, i, D, f);
+    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+    if (a.b) walk_other<DT>(a.b, 0, a.bdt, i, D, b);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      f[e] = fmaf((f[e] - mu) * rstd, a.w ? w[e] : 1.f, a.b ? b[e] : 0.f);
+    walk_store<DT>(a.y, yo, a.ydt, i, D, f);
   }
   if (threadIdx.x == 0 && a.mean) {
     a.mean[row] = mu;
@@ -96,45 +157,74 @@ __global__ __launch_bounds__(NT) void ln_fwd_long_kernel(const Fwd a) {
   }
 }
 
-__global__ __launch_bounds__(NT) void ln_bwd_long_kernel(const Bwd a) {
-  __shared__ float red[NT / 64];
-  const long long row = blockIdx.x, D = a.D;
-  const long long go = row * a.lddy, eo = row * a.ldds, so = row * a.lds, xo = row * D;
+template <int DT>
+__global__ __launch_bounds__(LT) void ln_bwd_long_kernel(const Bwd a) {
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>(), STEP = LT * V;
+  __shared__ float red[LT / 64];
+  const long long row = blockIdx.x, D = a.D, t0 = threadIdx.x * V;
+  const AS1 raw_t* s = gptr((const raw_t*)a.s) + row * a.lds;
   const float mu = a.mean[row], rstd = a.rstd[row];
   float c1 = 0.f, c2 = 0.f;
-  for (long long i = threadIdx.x; i < D; i += NT) {
-    float g = ld_any(a.dy, go + i, a.ydt);
-    if (a.w) g *= ld_any(a.w, i, a.wdt);
-    c1 += g;
-    c2 = fmaf(g, (ld_any(a.s, so + i, a.sdt) - mu) * rstd, c2);
+  for (long long i = t0; i < D; i += STEP) {
+    float g[V], h[V], w[V];
+    walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
+    walk_load<DT>(s, i, D, h);
+    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float v = a.w ? g[e] * w[e] : g[e];
+      c1 += v;
+      c2 = fmaf(v, (h[e] - mu) * rstd, c2);
+    }
   }
   c1 = block_sum(c1, red) / (float)D;
   c2 = block_sum(c2, red) / (float)D;
-  for (long long i = threadIdx.x; i < D; i += NT) {
-    float g = ld_any(a.dy, go + i, a.ydt);
-    if (a.w) g *= ld_any(a.w, i, a.wdt);
-    const float h = (ld_any(a.s, so + i, a.sdt) - mu) * rstd;
-    float d = rstd * (g - c1 - h * c2);
-    if (a.ds) d += ld_any(a.ds, eo + i, a.sdt);
-    st_any(a.dx, xo + i, a.sdt, d);
-    if (a.dz) st_any(a.dz, xo + i, a.zdt, d);
+  for (long long i = t0; i < D; i += STEP) {
+    float g[V], h[V], w[V], d[V];
+    walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
+    walk_load<DT>(s, i, D, h);
+    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+    if (a.ds) walk_load<DT>(gptr((const raw_t*)a.ds) + row * a.ldds, i, D, d);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float v = a.w ? g[e] * w[e] : g[e];
+      g[e] = rstd * (v - c1 - (h[e] - mu) * rstd * c2) + (a.ds ? d[e] : 0.f);
+    }
+    walk_store<DT>(a.dx, row * D, DT, i, D, g);
+    if (a.dz) walk_store<DT>(a.dz, row * D, a.zdt, i, D, g);
   }
 }
 
-// one column a thread over one chunk of rows: part[chunk][0 dw, 1 db][D]
+// V columns a thread over one chunk of rows: part[chunk][0 dw, 1 db][D]
+template <int DT>
 __global__ __launch_bounds__(NT) void ln_param_part_kernel(const Bwd a) {
-  const long long c = (long long)blockIdx.x * NT + threadIdx.x;
+  typedef typename DTypeTraits<DT>::raw_t raw_t;
+  constexpr int V = row_vec<DT>();
+  const long long c = ((long long)blockIdx.x * NT + threadIdx.x) * V;
   if (c >= a.D) return;
   const long long per = (a.rows + a.chunks - 1) / a.chunks;
   const long long r0 = blockIdx.y * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
-  float dw = 0.f, db = 0.f;
+  float dw[V], db[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
   for (long long r = r0; r < r1; ++r) {
-    const float g = ld_any(a.dy, r * a.lddy + c, a.ydt);
-    dw = fmaf(g, (ld_any(a.s, r * a.lds + c, a.sdt) - a.mean[r]) * a.rstd[r], dw);
-    db += g;
+    float g[V], h[V];
+    walk_other<DT>(a.dy, r * a.lddy, a.ydt, c, a.D, g);
+    walk_load<DT>(gptr((const raw_t*)a.s) + r * a.lds, c, a.D, h);
+    const float mu = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      dw[e] = fmaf(g[e], (h[e] - mu) * rstd, dw[e]);
+      db[e] += g[e];
+    }
   }
-  a.part[(2LL * blockIdx.y) * a.D + c] = dw;
-  a.part[(2LL * blockIdx.y + 1) * a.D + c] = db;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (c + e < a.D) {
+      a.part[2LL * blockIdx.y * a.D + c + e] = dw[e];
+      a.part[(2LL * blockIdx.y + 1) * a.D + c + e] = db[e];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -167,6 +257,19 @@ template <int TR> struct RowSum {      // sums over the TR threads of a row
     return r;
   }
 };
+
+// A thread's R accesses, issued back to back.  One that lies behind the row's
+// end for the whole wave is left out: a size class may be half empty.
+template <int DT, bool TAIL, bool STREAM, int R>
+__device__ __forceinline__ void load_all(const AS1 typename DTypeTraits<DT>::raw_t* row, int t0,
+                                         int step, int n, u32x4n* raw) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    raw[r] = (u32x4n)0u;
+    if (r == 0 || __builtin_amdgcn_readfirstlane(t0 + r * step) < n)
+      raw[r] = load_vec<DT, TAIL, STREAM>(row, t0 + r * step, n);
+  }
+}
 
 // E elements in one of the three types (uniform over the launch): the weights,
 // and z, dy, dz or y where their type is not the stream's.  V elements in
@@ -249,15 +352,15 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
     const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
     float f[E];
     u32x4n raw[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) raw[r] = load_vec<DT, TAIL>(x, t0 + r * step, D);
     if (a.z) {
       float g[E];
+      // x and z are read for the last time: s is what the backward pass reads
+      // (16384 x 4096 fp16: 104 -> 85 us)
+      load_all<DT, TAIL, true, R>(x, t0, step, D, raw);
       if (a.zdt == DT) {
         const AS1 raw_t* z = gptr((const raw_t*)a.z) + row * a.ldz;
         u32x4n zraw[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) zraw[r] = load_vec<DT, TAIL>(z, t0 + r * step, D);
+        load_all<DT, TAIL, true, R>(z, t0, step, D, zraw);
 #pragma unroll
         for (int r = 0; r < R; ++r)
           vec_to_f32<DT>(clip_vec<DT, TAIL>(zraw[r], t0 + r * step, D), g + r * V);
@@ -275,6 +378,7 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
         if (live) store_vec<DT, TAIL>(gptr((raw_t*)a.s) + row * D, i, D, f + r * V);
       }
     } else {
+      load_all<DT, TAIL, false, R>(x, t0, step, D, raw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(raw[r], t0 + r * step, D), f + r * V);
@@ -334,17 +438,12 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
     const AS1 raw_t* ds = gptr((const raw_t*)a.ds) + row * a.ldds;
     float h[E], g[E];
     u32x4n sraw[R], eraw[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) sraw[r] = load_vec<DT, TAIL>(s, t0 + r * step, D);
-    if (a.ds) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) eraw[r] = load_vec<DT, TAIL>(ds, t0 + r * step, D);
-    }
+    load_all<DT, TAIL, true, R>(s, t0, step, D, sraw);
+    if (a.ds) load_all<DT, TAIL, true, R>(ds, t0, step, D, eraw);
     if (a.ydt == DT) {
       const AS1 raw_t* dy = gptr((const raw_t*)a.dy) + row * a.lddy;
       u32x4n graw[R];
-#pragma unroll
-      for (int r = 0; r < R; ++r) graw[r] = load_vec<DT, TAIL>(dy, t0 + r * step, D);
+      load_all<DT, TAIL, true, R>(dy, t0, step, D, graw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(graw[r], t0 + r * step, D), g + r * V);
@@ -468,10 +567,15 @@ long long row_blocks(long long rows, long long D, long long cap) {
   return n < most ? n : most;
 }
 
-constexpr long long FWD_BLOCKS = 4096, BWD_BLOCKS = 1024;
+constexpr long long FWD_BLOCKS = 4096;
+// A workgroup leaves 8 D bytes of sums: fewer of them for longer rows (us with
+// 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 131072 x
+// 512 fp16 117 | 104, 1048576 x 64 fp16 186 | 142).  Rows of 1024 threads again
+// need 1024, a workgroup for every CU (8192 x 16384 fp16 342 | 224).
+long long bwd_blocks(long long D) { return D > 512 && D <= 8192 ? 512 : 1024; }
 
 int param_chunks(int dt, long long rows, long long D) {
-  if (!looped(dt, D)) return (int)row_blocks(rows, D, BWD_BLOCKS);
+  if (!looped(dt, D)) return (int)row_blocks(rows, D, bwd_blocks(D));
   const long long c = (rows + 63) / 64;
   return (int)(c < 512 ? c : 512);
 }
@@ -486,13 +590,17 @@ void launch_fwd(const Fwd& a, hipStream_t st) {
 }
 template <int DT, int TR, int E>
 void launch_bwd(const Bwd& a, hipStream_t st) {
-  const dim3 grid((unsigned)row_blocks(a.rows, a.D, BWD_BLOCKS)), block(RowSum<TR>::BT);
+  const dim3 grid((unsigned)row_blocks(a.rows, a.D, bwd_blocks(a.D))), block(RowSum<TR>::BT);
   if (a.D % row_vec<DT>())
     hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
   else
     hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, false>), grid, block, 0, st, a);
 }
 template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
+  if (looped(DT, a.D)) {
+    hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
+    return;
+  }
   const int n = row_threads(a.D);
   bool done = false;
 #define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_fwd<DT, TR, E>(a, st); done = true; }
@@ -500,6 +608,15 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
 #undef F
 }
 template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
+  if (looped(DT, a.D)) {
+    if (a.dx)
+      hipLaunchKernelGGL(ln_bwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
+    const long long cols = NT * row_vec<DT>();
+    if (a.part)
+      hipLaunchKernelGGL(ln_param_part_kernel<DT>,
+                         dim3((unsigned)((a.D + cols - 1) / cols), a.chunks), dim3(NT), 0, st, a);
+    return;
+  }
   const int n = row_threads(a.D);
   bool done = false;
 #define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_bwd<DT, TR, E>(a, st); done = true; }
@@ -524,14 +641,9 @@ KFAC_API int kfac_ln_forward(const KfacLnFwd* args, int bytes, hipStream_t strea
       !dtype_ok(a.ydt) || (a.z && (!a.s || !dtype_ok(a.zdt))) || (a.w && !dtype_ok(a.wdt)) ||
       (a.b && !dtype_ok(a.bdt)) || !a.mean != !a.rstd)
     return -2;
-  if (looped(a.sdt, a.D))
-    hipLaunchKernelGGL(ln_fwd_long_kernel, dim3((unsigned)a.rows), dim3(NT), 0, stream, a);
-  else if (a.sdt == KDT_F32)
-    launch_fwd_any<KDT_F32>(a, stream);
-  else if (a.sdt == KDT_BF16)
-    launch_fwd_any<KDT_BF16>(a, stream);
-  else
-    launch_fwd_any<KDT_F16>(a, stream);
+  if (a.sdt == KDT_F32) launch_fwd_any<KDT_F32>(a, stream);
+  else if (a.sdt == KDT_BF16) launch_fwd_any<KDT_BF16>(a, stream);
+  else launch_fwd_any<KDT_F16>(a, stream);
   return (int)hipGetLastError();
 }
 
@@ -547,18 +659,9 @@ KFAC_API int kfac_ln_backward(const KfacLnBwd* args, int bytes, hipStream_t stre
     return -2;
   if (!a.dw && !a.db) a.part = nullptr;
   a.chunks = param_chunks(a.sdt, a.rows, a.D);
-  if (looped(a.sdt, a.D)) {
-    if (a.dx) hipLaunchKernelGGL(ln_bwd_long_kernel, dim3((unsigned)a.rows), dim3(NT), 0, stream, a);
-    if (a.part)
-      hipLaunchKernelGGL(ln_param_part_kernel, dim3((unsigned)((a.D + NT - 1) / NT), a.chunks),
-                         dim3(NT), 0, stream, a);
-  } else if (a.sdt == KDT_F32) {
-    launch_bwd_any<KDT_F32>(a, stream);
-  } else if (a.sdt == KDT_BF16) {
-    launch_bwd_any<KDT_BF16>(a, stream);
-  } else {
-    launch_bwd_any<KDT_F16>(a, stream);
-  }
+  if (a.sdt == KDT_F32) launch_bwd_any<KDT_F32>(a, stream);
+  else if (a.sdt == KDT_BF16) launch_bwd_any<KDT_BF16>(a, stream);
+  else launch_bwd_any<KDT_F16>(a, stream);
   if (a.part)
     hipLaunchKernelGGL(ln_param_sum_kernel, dim3((unsigned)((a.D + 31) / 32)), dim3(1024), 0,
                        stream, a);

@@ -65,12 +65,14 @@ template <int DT> __device__ __forceinline__ u32x4n vec_shift(u32x4n v, int s) {
 // issued back to back: an access past the end is moved into the row -- one that
 // holds the end (TAIL: n need not be a multiple of V) to the row's last V
 // elements, to be shifted down.
-template <int DT, bool TAIL>
+// STREAM: the row is not read again soon (non-temporal).
+template <int DT, bool TAIL, bool STREAM = false>
 __device__ __forceinline__ u32x4n load_vec(const AS1 typename DTypeTraits<DT>::raw_t* row, int i,
                                            int n) {
   constexpr int V = row_vec<DT>();
   const int at = i + V <= n ? i : TAIL && i < n ? n - V : 0;
-  return *(const AS1 u32x4u*)(row + at);
+  const AS1 u32x4u* p = (const AS1 u32x4u*)(row + at);
+  return STREAM ? __builtin_nontemporal_load(p) : *p;
 }
 template <int DT, bool TAIL>
 __device__ __forceinline__ u32x4n clip_vec(u32x4n v, int i, int n) {

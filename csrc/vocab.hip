@@ -15,7 +15,7 @@
 //
 // Forward: ONE pass over the row.  A thread keeps the running maximum m of its
 // elements, s = sum exp((x - m) / T) and a = sum exp((x - m) / T) (x - m) / T, each
-// brought to a new maximum once per tile of four 16-byte loads; the threads'
+// brought to a new maximum once per tile of 16 elements; the threads'
 // (m, s, a) are joined at the end.  The alternatives need no second pass: the
 // k-th largest of the threads' maxima is a bound that at least k elements
 // reach, and only the threads that reach it have such elements, so about k of
@@ -44,7 +44,7 @@ struct KfacVocabFwd {
   float* keep_q;
   void* ws;
   long long ld, rows, V, ignore;
-  int dt, k, K, tdt;
+  int dt, k, K, tdt, stream;
   float inv_t;
 };
 
@@ -70,6 +70,11 @@ typedef KfacVocabBwd Bwd;
 constexpr int TOP_MAX = 128;      // alternatives, and slots of a teacher's row
 constexpr int MAX_V = 1 << 30;    // elements of a row: 32-bit offsets within it
 constexpr int MAX_SPLITS = 64;    // workgroups a row
+// Logits that the 256 MB of last-level cache cannot hold beside their gradient
+// are read past it (non-temporal): the backward pass would not find them there.
+// us forward + backward, streamed | not: 4096 x 131072 bf16 197 + 373 | 232 +
+// 351, 2048 x 32064 fp32 47 + 88 | 70 + 77, 700 x 10000 fp32 12 + 13 | 12 + 12.
+constexpr long long STREAM_FROM = 128LL << 20;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // An exponent far below what exp2 gives 0 for, whose product with that 0 is 0.
 constexpr float LOWEST = -1e9f;
@@ -142,11 +147,25 @@ __device__ __forceinline__ void fetch(const AS1 typename DTypeTraits<DT>::raw_t*
     if (i + e >= end) f[e] = -INFINITY;
 }
 
-// The running (m, s, a) of one thread over a tile of N elements: s = sum e^(..),
+// The running (m, s, a) of one thread over N more elements: s = sum e^(..),
 // a = sum e^(..) u with u = (x - m) / T in units of log 2.  c1 = log2 e / T.
+// Both return the elements' maximum.
 template <int N, bool ENT>
-__device__ __forceinline__ void fold_any(const float* f, float top, float c1, float& s, float& a) {
-  const float base = top == -INFINITY ? 0.f : top;
+__device__ __forceinline__ float raise(const float* f, float c1, float& m, float& s, float& a) {
+  float tile = f[0];
+#pragma unroll
+  for (int e = 1; e < N; ++e) tile = fmaxf(tile, f[e]);
+  const float top = fmaxf(m, tile);
+  const float back = fmaxf((m - (top == -INFINITY ? 0.f : top)) * c1, LOWEST);
+  const float scale = __builtin_amdgcn_exp2f(back);
+  if (ENT) a = scale * fmaf(back, s, a);
+  s *= scale;
+  m = top;
+  return tile;
+}
+template <int N, bool ENT>
+__device__ __forceinline__ void add_any(const float* f, float c1, float m, float& s, float& a) {
+  const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const float u = (f[e] - base) * c1, x = __builtin_amdgcn_exp2f(u);
@@ -154,25 +173,22 @@ __device__ __forceinline__ void fold_any(const float* f, float top, float c1, fl
     if (ENT) a = fmaf(x, fmaxf(u, LOWEST), a);        // exp(-inf) = 0 times a finite number
   }
 }
-
+template <int N, bool ENT>
+__device__ __forceinline__ float fold_any(const float* f, float c1, float& m, float& s, float& a) {
+  const float tile = raise<N, ENT>(f, c1, m, s, a);
+  add_any<N, ENT>(f, c1, m, s, a);
+  return tile;
+}
 // The same with one instruction less an element, u' = x c1 - R with R = m c1
 // rounded: every u' of the tile is off by the same d = m c1 - R, which is known
 // exactly and taken out of the sums.  Not where R is so large that d is no
 // small number (or no number), and not where an entropy's product meets a -inf.
 template <int N, bool ENT>
-__device__ __forceinline__ void fold(const float* f, float c1, float& m, float& s, float& a) {
-  float top = m;
-#pragma unroll
-  for (int e = 0; e < N; ++e) top = fmaxf(top, f[e]);
-  // the running sums brought to the new maximum
-  const float back = fmaxf((m - (top == -INFINITY ? 0.f : top)) * c1, LOWEST);
-  const float scale = __builtin_amdgcn_exp2f(back);
-  if (ENT) a = scale * fmaf(back, s, a);
-  s *= scale;
-  m = top;
-  const float R = top * c1;
-  float st = 0.f, at = 0.f;
+__device__ __forceinline__ float fold(const float* f, float c1, float& m, float& s, float& a) {
+  const float tile = raise<N, ENT>(f, c1, m, s, a);
+  const float R = m * c1;
   if (!__any(!(fabsf(R) < 0x1p20f))) {
+    float st = 0.f, at = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float u = fmaf(f[e], c1, -R), x = __builtin_amdgcn_exp2f(u);
@@ -180,40 +196,82 @@ __device__ __forceinline__ void fold(const float* f, float c1, float& m, float& 
       if (ENT) at = fmaf(x, u, at);
     }
     if (!ENT || !__any(at != at)) {
-      const float d = fmaf(top, c1, -R), fix = __builtin_amdgcn_exp2f(-d);
+      const float d = fmaf(m, c1, -R), fix = __builtin_amdgcn_exp2f(-d);
       s = fmaf(st, fix, s);
       if (ENT) a = fmaf(fmaf(-d, st, at), fix, a);
-      return;
+      return tile;
     }
   }
-  fold_any<N, ENT>(f, top, c1, s, a);
+  add_any<N, ENT>(f, c1, m, s, a);
+  return tile;
 }
 
-template <int DT, int NT, bool ENT>
-__device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* x, int begin,
-                                     int end, int n, float c1, float& m, float& s, float& a) {
-  constexpr int V = row_vec<DT>(), U = 4, STEP = NT * V;
+// How a workgroup walks a chunk of a row: whole 16-byte lines from the first
+// one on, element head + (j NT + thread) V in access j; the fewer than V
+// elements before that line are the last thread's.  (Accesses at odd multiples of
+// two bytes are slow: 8192 x 50001 bf16 185 us against 133 us for 50000.)
+template <int DT> struct Walk {
+  int begin, end, n, head;        // chunk, row's length, first line's element
+  template <class P> __device__ __forceinline__ Walk(P x, int b, int e, int len) {
+    constexpr int V = row_vec<DT>(), ES = 16 / V;
+    const int past = (int)(((uintptr_t)(x + b) & 15) / ES);
+    begin = b;
+    end = e;
+    n = len;
+    head = past ? b + V - past : b;
+    if (head > e) head = e;
+  }
+};
+
+// A tile is 16 elements a thread (bf16 32 | 16: 8192 x 50001 with entropy 180 |
+// 160 us, 32768 x 2000 42 | 33, 4096 x 131072 182 | 186).  Of the largest values of
+// a thread's elements SLOTS are kept, each of a run of tiles.
+constexpr int SLOTS = 8;
+
+template <int DT, int NT, bool ENT, bool TOP>
+__device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* x,
+                                     const Walk<DT> w, bool stream, float c1, int shift,
+                                     float (*slot)[NT], float& m, float& s, float& a) {
+  constexpr int V = row_vec<DT>(), U = 16 / V, STEP = NT * V;
   m = -INFINITY;
   s = a = 0.f;
-  int at = begin;
-  for (; at + U * STEP <= end; at += U * STEP) {
-    const int i = at + threadIdx.x * V;
-    u32x4n raw[U];
+  float run = -INFINITY;
+  int tile = 0, at = w.head;
+  // two loops: one with a choice of loads in it ends with plain ones in both
+  auto tiles = [&](auto load) {
+    for (; at + U * STEP <= w.end; at += U * STEP, ++tile) {
+      const AS1 u32x4u* p = (const AS1 u32x4u*)(x + at + threadIdx.x * V);
+      u32x4n raw[U];
+      float f[U * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = load(p + u * NT);
+#pragma unroll
+      for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
+      const float top = fold<U * V, ENT>(f, c1, m, s, a);
+      if (TOP) {
+        run = fmaxf(run, top);
+        if (((tile + 1) & ((1 << shift) - 1)) == 0) {
+          slot[tile >> shift][threadIdx.x] = run;
+          run = -INFINITY;
+        }
+      }
+    }
+  };
+  if (stream) tiles([](const AS1 u32x4u* p) -> u32x4n { return __builtin_nontemporal_load(p); });
+  else tiles([](const AS1 u32x4u* p) -> u32x4n { return *p; });
+  // what is left, fewer than U accesses a thread, and what lies before the first line
+  const bool first = threadIdx.x == NT - 1 && w.head > w.begin;
+  float before[V];
+  if (first) fetch<DT>(x, w.begin, w.head, w.n, before);
+  if (at < w.end) {
     float f[U * V];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      raw[u] = __builtin_nontemporal_load((const AS1 u32x4u*)(x + i + u * STEP));
-#pragma unroll
-    for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
-    fold<U * V, ENT>(f, c1, m, s, a);
+      fetch<DT>(x, at + threadIdx.x * V + u * STEP, w.end, w.n, f + u * V);
+    run = fmaxf(run, fold_any<U * V, ENT>(f, c1, m, s, a));
   }
-  if (at < end) {
-    const int i = at + threadIdx.x * V;
-    float f[U * V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) fetch<DT>(x, i + u * STEP, end, n, f + u * V);
-    fold<U * V, ENT>(f, c1, m, s, a);
-  }
+  if (TOP) slot[tile >> shift][threadIdx.x] = run;
+  if (first) fold_any<V, ENT>(before, c1, m, s, a);
 }
 
 // (m, s, a) joined over the workgroup
@@ -227,100 +285,150 @@ __device__ __forceinline__ void join(float c1, float* red, float& m, float& s, f
   m = M;
 }
 
-// The threads that hold elements are fewer than k only where the chunk is one
-// access a thread: then all its elements, at most k V of them, are candidates.
 template <int NT> struct TopShared {
   static constexpr int CAND = 4 * NT;
   uint64_t cand[CAND];
+  static constexpr int LIST = 2 * NT;   // slots to be read again
+  union {
+    float slot[SLOTS][NT];
+    uint64_t kept[CAND];
+  };
   uint32_t key[NT];
-  int list[NT];
+  union {
+    unsigned short list[LIST];
+    int ties[NT];
+  };
   int hist[256];
-  int n, winners, bound;
+  int n, entries, bound;
 };
+
+// The largest bound that at least k of a wave's N keys a lane reach, bit by bit
+// from the top; 0 where there are fewer.  Keys equal above bit LOW are equal.
+template <int N, int LOW>
+__device__ __forceinline__ uint32_t kth_of_wave(const uint32_t* own, int k) {
+  uint32_t bound = 0;
+  for (int bit = 31; bit >= LOW; --bit) {
+    const uint32_t next = bound | 1u << bit;
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) count += __popcll(__ballot(own[j] >= next));
+    if (count >= k) bound = next;
+  }
+  return bound;
+}
 
 // The k largest (value, lower index) of a chunk of a row as full keys, largest
 // first, handed to out(rank, key); fewer than k elements give fewer.  m, s: the
-// calling thread's running maximum and sum.
+// calling thread's running maximum and sum; sh.slot: its tiles' maxima, 2^shift
+// tiles a slot.
+//
+// The k-th largest of the threads' maxima bounds the k-th largest element from
+// below, and whatever reaches it lies in a slot whose maximum does: about k
+// slots of all the 8 NT are read again.  (Every element is a candidate where
+// fewer than k threads have any: at most k V of them.)
 template <int DT, int NT, class Out>
 __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>::raw_t* x,
-                                             int begin, int end, int n, float m, float s, int k,
+                                             const Walk<DT> w, float m, float s, int k, int shift,
                                              TopShared<NT>& sh, Out out) {
   constexpr int V = row_vec<DT>(), STEP = NT * V;
   // low bits of a key that say nothing: bf16 fills 16 bits of an fp32, fp16 19
   constexpr int LOW = DT == KDT_F32 ? 0 : DT == KDT_BF16 ? 16 : 8;
-  const int tid = threadIdx.x, mine = begin + tid * V, per = (end - begin + STEP - 1) / STEP;
-  // this thread's largest key; a NaN or +inf made s NaN, the maximum passes over NaN
-  uint32_t key = mine < end ? order_key(m) : 0u;
-  if (s != s) {
-    key = 0;
-    for (int j = 0; j < per; ++j) {
+  const int tid = threadIdx.x, mine = w.head + tid * V;
+  const int per = (w.end - w.head + STEP - 1) / STEP;        // accesses a thread at most
+  const bool first = tid == NT - 1 && w.head > w.begin;      // has the elements before the lines
+  // visit(f, i, e1): elements i .. e1 - 1 of this thread, access by access
+  auto each = [&](int j0, int j1, auto visit) {
+    for (int j = j0; j < j1 && mine + j * STEP < w.end; ++j) {
       float f[V];
       const int i = mine + j * STEP;
-      if (i >= end) break;
-      fetch<DT>(x, i, end, n, f);
+      fetch<DT>(x, i, w.end, w.n, f);
+      visit(f, i, w.end);
+    }
+  };
+  auto before = [&](auto visit) {
+    if (first) {
+      float f[V];
+      fetch<DT>(x, w.begin, w.head, w.n, f);
+      visit(f, w.begin, w.head);
+    }
+  };
+  // this thread's largest key; a NaN or +inf made s NaN, the maximum passes over NaN
+  uint32_t key = mine < w.end || first ? order_key(m) : 0u;
+  if (s != s) {
+    key = 0;
+    auto most = [&](const float* f, int i, int e1) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const uint32_t o = i + e < end ? order_key(f[e]) : 0u;
+        const uint32_t o = i + e < e1 ? order_key(f[e]) : 0u;
         key = o > key ? o : key;
       }
-    }
+    };
+    each(0, per, most);
+    before(most);
   }
   sh.key[tid] = key;
-  if (tid == 0) sh.n = sh.winners = 0;
+  if (tid == 0) sh.n = sh.entries = 0;
   __syncthreads();
-  // the k-th largest of the threads' keys, bit by bit (0 where there are fewer)
   if (tid < 64) {
-    uint32_t own[NT / 64], bound = 0;
+    uint32_t own[NT / 64];
 #pragma unroll
     for (int j = 0; j < NT / 64; ++j) own[j] = sh.key[tid + 64 * j];
-    for (int bit = 31; bit >= LOW; --bit) {
-      const uint32_t next = bound | 1u << bit;
-      int count = 0;
-#pragma unroll
-      for (int j = 0; j < NT / 64; ++j) count += __popcll(__ballot(own[j] >= next));
-      if (count >= k) bound = next;
-    }
+    const uint32_t bound = kth_of_wave<NT / 64, LOW>(own, k);
     if (tid == 0) sh.bound = (int)bound;
   }
   __syncthreads();
   const uint32_t bound = (uint32_t)sh.bound ? (uint32_t)sh.bound : 1u;
-  if (key >= bound) sh.list[atomicAdd(&sh.winners, 1)] = tid;
-  __syncthreads();
-  const int items = sh.winners * per;
-  for (int it = tid; it < items; it += NT) {
-    const int w = it / per, i = begin + sh.list[w] * V + (it - w * per) * STEP;
-    if (i >= end) continue;
-    float f[V];
-    fetch<DT>(x, i, end, n, f);
+  auto take = [&](const float* f, int i, int e1) {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (i + e < end && order_key(f[e]) >= bound) {
+      if (i + e < e1 && order_key(f[e]) >= bound) {
         const int c = atomicAdd(&sh.n, 1);
         if (c < TopShared<NT>::CAND) sh.cand[c] = full_key(f[e], (uint32_t)(i + e));
       }
+  };
+  const int lines = (V == 4 ? 2 : 1) + shift;      // log2 of a slot's accesses
+  if (key >= bound) {
+    for (int q = 0; q < SLOTS && q << lines < per; ++q)
+      if (s != s || order_key(sh.slot[q][tid]) >= bound) {
+        const int c = atomicAdd(&sh.entries, 1);
+        if (c < TopShared<NT>::LIST) sh.list[c] = (unsigned short)(q * NT + tid);
+      }
+    before(take);
   }
   __syncthreads();
-  if (sh.n > TopShared<NT>::CAND) {
+  // the slots' accesses shared out over the workgroup: one round trip, as a rule
+  const int entries = sh.entries;
+  if (entries <= TopShared<NT>::LIST) {
+    for (int it = tid; it < entries << lines; it += NT) {
+      const int at = sh.list[it >> lines], q = at / NT;
+      const int i = w.head + (at % NT) * V + ((q << lines) + (it & ((1 << lines) - 1))) * STEP;
+      if (i < w.end) {
+        float f[V];
+        fetch<DT>(x, i, w.end, w.n, f);
+        take(f, i, w.end);
+      }
+    }
+  }
+  __syncthreads();
+  if (sh.n > TopShared<NT>::CAND || entries > TopShared<NT>::LIST) {
     // Too many equal or crowded values: the k-th largest key exactly, by counting
     // its digits from the top; then the larger ones and, in the order of their
     // indices, as many equal ones as are wanted -- k in all.
     int need = k;
     uint32_t prefix = 0;
-    for (int shift = 24; shift >= LOW; shift -= 8) {
+    for (int shift_d = 24; shift_d >= LOW; shift_d -= 8) {
       for (int j = tid; j < 256; j += NT) sh.hist[j] = 0;
       __syncthreads();
-      for (int j = 0; j < per; ++j) {
-        float f[V];
-        const int i = mine + j * STEP;
-        if (i >= end) break;
-        fetch<DT>(x, i, end, n, f);
+      auto count = [&](const float* f, int i, int e1) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const uint32_t o = order_key(f[e]);
-          if (i + e < end && (uint64_t)o >> (shift + 8) == prefix)
-            atomicAdd(&sh.hist[(o >> shift) & 255], 1);
+          if (i + e < e1 && (uint64_t)o >> (shift_d + 8) == prefix)
+            atomicAdd(&sh.hist[(o >> shift_d) & 255], 1);
         }
-      }
+      };
+      each(0, per, count);
+      before(count);
       __syncthreads();
       int digit = 255, left = need;
       while (digit > 0 && sh.hist[digit] < left) left -= sh.hist[digit--];
@@ -331,41 +439,41 @@ __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>:
     const uint32_t low = LOW ? (1u << LOW) - 1u : 0u, kth = prefix << LOW;   // of the digits counted
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    for (int j = 0; j < per; ++j) {
-      float f[V];
-      const int i = mine + j * STEP;
-      if (i >= end) break;
-      fetch<DT>(x, i, end, n, f);
+    auto larger = [&](const float* f, int i, int e1) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (i + e < end && order_key(f[e]) > (kth | low))
+        if (i + e < e1 && order_key(f[e]) > (kth | low))
           sh.cand[atomicAdd(&sh.n, 1)] = full_key(f[e], (uint32_t)(i + e));
-    }
+    };
+    each(0, per, larger);
+    before(larger);
     __syncthreads();
+    // equal ones in the order of their indices: V a thread from the chunk's begin on
     int have = sh.n;                       // k - need
-    for (int at = begin; at < end && have < k; at += STEP) {
+    for (int at = w.begin; at < w.end && have < k; at += STEP) {
       float f[V];
       const int i = at + tid * V;
       int mine_n = 0;
-      if (i < end) {
-        fetch<DT>(x, i, end, n, f);
+      if (i < w.end) {
+        fetch<DT>(x, i, w.end, w.n, f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) mine_n += i + e < end && (order_key(f[e]) | low) == (kth | low);
+        for (int e = 0; e < V; ++e)
+          mine_n += i + e < w.end && (order_key(f[e]) | low) == (kth | low);
       }
       __syncthreads();
-      sh.list[tid] = mine_n;
+      sh.ties[tid] = mine_n;
       __syncthreads();
-      int before = have, all = have;
+      int rank = have, all = have;
       for (int j = 0; j < NT; ++j) {
-        before += j < tid ? sh.list[j] : 0;
-        all += sh.list[j];
+        rank += j < tid ? sh.ties[j] : 0;
+        all += sh.ties[j];
       }
       if (mine_n) {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-          if (i + e < end && (order_key(f[e]) | low) == (kth | low)) {
-            if (before < k) sh.cand[before] = full_key(f[e], (uint32_t)(i + e));
-            ++before;
+          if (i + e < w.end && (order_key(f[e]) | low) == (kth | low)) {
+            if (rank < k) sh.cand[rank] = full_key(f[e], (uint32_t)(i + e));
+            ++rank;
           }
       }
       have = all;
@@ -374,11 +482,35 @@ __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>:
     if (tid == 0) sh.n = k;
     __syncthreads();
   }
-  const int count = sh.n;
+  // Their order by counting, for each, the larger ones: quadratic, so that of many
+  // those below the k-th are dropped first (65536 x 512 bf16 with 128 of them 1871
+  // -> 888 us; with 300 candidates, 32768 x 2000, it would be 286 -> 483 us).
+  int count = sh.n;
+  const uint64_t* cand = sh.cand;
+  if (count > 400) {
+    if (tid < 64) {
+      uint32_t own[TopShared<NT>::CAND / 64];
+#pragma unroll
+      for (int j = 0; j < TopShared<NT>::CAND / 64; ++j)
+        own[j] = tid + 64 * j < count ? (uint32_t)(sh.cand[tid + 64 * j] >> 32) : 0u;
+      const uint32_t kth = kth_of_wave<TopShared<NT>::CAND / 64, LOW>(own, k);
+      if (tid == 0) {
+        sh.bound = (int)kth;
+        sh.n = 0;
+      }
+    }
+    __syncthreads();
+    const uint32_t kth = (uint32_t)sh.bound;
+    for (int c = tid; c < count; c += NT)
+      if ((uint32_t)(sh.cand[c] >> 32) >= kth) sh.kept[atomicAdd(&sh.n, 1)] = sh.cand[c];
+    __syncthreads();
+    count = sh.n;
+    cand = sh.kept;
+  }
   for (int c = tid; c < count; c += NT) {
-    const uint64_t v = sh.cand[c];
+    const uint64_t v = cand[c];
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += sh.cand[j] > v;
+    for (int j = 0; j < count; ++j) rank += cand[j] > v;
     if (rank < k) out(rank, v);
   }
 }
@@ -488,11 +620,14 @@ __device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M
   a.stats[2 * row + 1] = L;
 }
 
+// (Six waves a SIMD also where both entropy and alternatives want registers:
+// 8192 x 50001 bf16 with 32 of them 189 -> 177 us.  Without either it costs.)
 template <int DT, int NT, int MODE, bool ENT, bool TOP>
-__global__ __launch_bounds__(NT) void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 256 && ENT && TOP ? 6 : 1)))
+void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
   __shared__ float red[NT / 64];
-  __shared__ TopShared<TOP ? NT : 1> tops;
+  __shared__ TopShared<TOP ? NT : 1> tops;        // without TOP a few bytes that nobody reads
   const long long row = blockIdx.x / splits;
   const int part = blockIdx.x % splits, n = (int)a.V;
   const int begin = part * chunk, end = n - begin < chunk ? n : begin + chunk;
@@ -516,8 +651,12 @@ __global__ __launch_bounds__(NT) void vocab_fwd_kernel(const Fwd a, int splits, 
     return;
   }
   const float c1 = a.inv_t * LOG2E;
+  const Walk<DT> w(x, begin, end, n);
+  // tiles a slot: the least power of two that leaves no more than SLOTS of them
+  const int tiles = (end - w.head) / (NT * 16) + 1;
+  const int shift = tiles <= SLOTS ? 0 : 32 - __clz((tiles - 1) / SLOTS);
   float m, s, sum;
-  scan<DT, NT, ENT>(x, begin, end, n, c1, m, s, sum);
+  scan<DT, NT, ENT, TOP>(x, w, a.stream, c1, shift, (float(*)[NT])tops.slot, m, s, sum);
   float M = m, S = s;
   join<NT, ENT>(c1, red, M, S, sum);
   if (splits > 1) {
@@ -527,7 +666,7 @@ __global__ __launch_bounds__(NT) void vocab_fwd_kernel(const Fwd a, int splits, 
       uint64_t* keys = (uint64_t*)((Part*)a.ws + a.rows * splits) + (row * splits + part) * a.k;
       for (int j = threadIdx.x; j < a.k; j += NT)
         if (j >= end - begin) keys[j] = 0;         // fewer elements than k
-      top_of_chunk<DT, NT>(x, begin, end, n, m, s, a.k, tops,
+      top_of_chunk<DT, NT>(x, w, m, s, a.k, shift, tops,
                            [&](int rank, uint64_t key) { keys[rank] = key; });
     }
     return;
@@ -539,7 +678,7 @@ __global__ __launch_bounds__(NT) void vocab_fwd_kernel(const Fwd a, int splits, 
     float L;
     logprob_row<DT, NT>(a, row, M, S, sum, L);
     if constexpr (TOP) {
-      top_of_chunk<DT, NT>(x, begin, end, n, m, s, a.k, tops, [&](int rank, uint64_t key) {
+      top_of_chunk<DT, NT>(x, w, m, s, a.k, shift, tops, [&](int rank, uint64_t key) {
         a.top_ids[row * a.k + rank] = (uint32_t)~(uint32_t)key;
         a.top_lp[row * a.k + rank] = log_prob(key_value((uint32_t)(key >> 32)), M, L, a.inv_t);
       });
@@ -633,10 +772,14 @@ __global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int spli
   typedef typename DTypeTraits<DT>::raw_t raw_t;
   constexpr int V = row_vec<DT>(), U = 4, STEP = BWD_NT * V, CHUNK = bwd_chunk<DT>();
   const long long row = blockIdx.x / splits;
-  const int n = (int)a.V, begin = blockIdx.x % splits * CHUNK;
-  const int end = n - begin < CHUNK ? n : begin + CHUNK;
+  const int n = (int)a.V, part = blockIdx.x % splits;
   const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ld;
   AS1 raw_t* dx = gptr((raw_t*)a.dx) + row * a.V;
+  // whole 16-byte lines of dx; the first workgroup has what lies before them, too
+  const int past = (int)(((uintptr_t)dx & 15) / (16 / V));
+  const int head = past && V - past < n ? V - past : past ? n : 0;
+  const int from = head + part * CHUNK, begin = part ? from : 0;
+  const int end = n - from < CHUNK ? n : from + CHUNK;
   const float M = a.stats[2 * row], L = a.stats[2 * row + 1];
   const long long tgt = MODE == LOGPROB && a.targets ? a.targets[row] : 0;
   const bool zero = M == -INFINITY || (MODE == LOGPROB && a.targets && tgt == a.ignore);
@@ -650,7 +793,10 @@ __global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int spli
     const float lp = (xi - M) * a.inv_t - L, p = __builtin_amdgcn_exp2f(lp * LOG2E);
     return ENT ? p * fmaf(ghs, fmaxf(lp, LOWEST) + H, gs) : p * gs;
   };
-  for (int at = begin; at < end; at += U * STEP) {
+  if (part == 0 && threadIdx.x < head)
+    dx[threadIdx.x] = DTypeTraits<DT>::from_f32(
+        zero ? 0.f : value(DTypeTraits<DT>::to_f32(x[threadIdx.x])));
+  for (int at = from; at < end; at += U * STEP) {
     const int i = at + threadIdx.x * V;
     float f[U * V];
     if (zero) {
@@ -689,17 +835,20 @@ __global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int spli
   }
 }
 
-// Threads a workgroup: a wave where a row is at most eight 16-byte accesses a
-// lane and its alternatives are fewer than half the lanes.
-int fwd_threads(int dt, long long V, int k) {
+// Threads a workgroup.  A row of at most 8 accesses a lane is a wave's; with
+// enough rows to fill the chip by waves, one of 32 is, too, and saves the
+// workgroup's barriers (us with 64 | 256: 32768 x 8000 bf16 99 | 113, with
+// entropy 101 | 155; 16384 x 16000 with entropy 103 | 118; but 700 x 10000 fp32
+// 42 | 22).  Half of a wave's lanes have to be more than the alternatives.
+int fwd_threads(int dt, long long rows, long long V, int k) {
   const int vec = dt == KDT_F32 ? 4 : 8;
-  return V <= 64 * vec * 8 && k <= 32 ? 64 : 256;
+  return k <= 32 && V <= 64 * vec * (rows >= 4096 ? 32 : 8) ? 64 : 256;
 }
 
 // Workgroups a row: enough to have four for every CU, but none with less than
 // two 16-byte accesses a thread.
 int fwd_splits(int dt, long long rows, long long V, int k) {
-  if (fwd_threads(dt, V, k) == 64) return 1;
+  if (fwd_threads(dt, rows, V, k) == 64) return 1;
   const long long least = 256LL * (dt == KDT_F32 ? 4 : 8) * 2, most = (V + least - 1) / least;
   long long n = (1024 + rows - 1) / rows;
   if (n > most) n = most;
@@ -712,7 +861,7 @@ bool dtype_ok(int dt) { return dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16;
 template <int DT, int MODE, bool ENT, bool TOP>
 void launch_fwd(const Fwd& a, hipStream_t st) {
   const int splits = fwd_splits(a.dt, a.rows, a.V, a.k);
-  if (splits == 1 && fwd_threads(a.dt, a.V, a.k) == 64) {
+  if (splits == 1 && fwd_threads(a.dt, a.rows, a.V, a.k) == 64) {
     hipLaunchKernelGGL((vocab_fwd_kernel<DT, 64, MODE, ENT, TOP>), dim3((unsigned)a.rows),
                        dim3(64), 0, st, a, 1, (int)a.V);
     return;
@@ -760,7 +909,7 @@ KFAC_API long long kfac_vocab_ws_bytes(int dt, long long rows, long long V, int 
 // alternatives.  Distillation: loss set, with ids, teacher, keep_ids, keep_q.
 KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t stream) {
   if (bytes != (int)sizeof(Fwd)) return -2;
-  const Fwd a = *args;
+  Fwd a = *args;
   if (!a.x || a.rows <= 0 || a.V <= 0 || a.V > MAX_V || a.rows > 0x7fffffffLL / MAX_SPLITS ||
       !(a.inv_t > 0.f) || !dtype_ok(a.dt) || !a.stats)
     return -2;
@@ -770,6 +919,7 @@ KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t
                    (a.k && (!a.top_lp || !a.top_ids)))
     return -2;
   if (!a.ws && kfac_vocab_ws_bytes(a.dt, a.rows, a.V, a.k)) return -2;
+  a.stream = a.rows * a.V * (a.dt == KDT_F32 ? 4 : 2) > STREAM_FROM;
   if (a.dt == KDT_F32) launch_fwd_any<KDT_F32>(a, stream);
   else if (a.dt == KDT_BF16) launch_fwd_any<KDT_BF16>(a, stream);
   else launch_fwd_any<KDT_F16>(a, stream);

@@ -34,7 +34,7 @@ _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # csrc/commo
 _GPU_TYPES = tuple(_CODE)
 
 # csrc/vocab.hip KfacVocabFwd, KfacVocabBwd
-_fwd = _lib.PackedCall('kfac_vocab_forward', '13P4q4if0P')
+_fwd = _lib.PackedCall('kfac_vocab_forward', '13P4q5if0P')
 _bwd = _lib.PackedCall('kfac_vocab_backward', '9P6q2if0P')
 
 
@@ -170,7 +170,7 @@ class _TokenLogprobs(torch.autograd.Function):
             stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
             ws, wp = _workspace(code, rows, V, k, dev)
             _fwd(dev, x.data_ptr(), _ptr(tgt), _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti),
-                 stats.data_ptr(), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, inv_t)
+                 stats.data_ptr(), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, 0, inv_t)
         else:
             x, M, L, all_lp = _cpu_stats(logits.reshape(rows, V), inv_t)
             skip = torch.zeros(rows, dtype=torch.bool) if tgt is None else \
@@ -297,7 +297,8 @@ class _TopkDistill(torch.autograd.Function):
             ws, wp = _workspace(code, rows, V, 0, dev)
             _fwd(dev, x.data_ptr(), 0, 0, 0, 0, 0, stats.data_ptr(), ids.data_ptr(),
                  teacher.data_ptr(), loss.data_ptr(), at.data_ptr(), mass.data_ptr(), wp, ld, rows,
-                 V, 0, code, 0, K, _CODE[teacher.dtype], inv_t)
+                 V, 0, code, 0, K, _CODE[teacher.dtype], 0,
+                 inv_t)
         elif rows:
             lp = _cpu_stats(logits.reshape(rows, V), inv_t)[3]
             some, at, q, logq = _cpu_teacher(ids.reshape(rows, K), teacher.reshape(rows, K), V,

@@ -69,6 +69,13 @@ def _rows(t, rows, D):
     return t, t.data_ptr(), ld, _CODE[t.dtype]
 
 
+def _like(t, dtype=None):
+    """An uninitialised contiguous tensor of t's shape."""
+    if dtype is None or dtype == t.dtype:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _vector(p):
     """(weight or bias contiguous, its address, its type's code); zeros for None."""
     if p is None:
@@ -84,21 +91,20 @@ def _forward(x, z, weight, bias, D, eps, ydtype, keep):
         x, z = z, x                              # the sum's type is the wider one's: fp32 ...
         if x.dtype != torch.float32:
             x = x.float()                        # ... also for bf16 + fp16
-    dtype, dev, shape = x.dtype, x.device, x.shape
-    y = torch.empty(shape, dtype=ydtype or dtype, device=dev)
+    y = _like(x, ydtype)
     s, sp = x, 0
     if z is not None:
-        s = torch.empty(shape, dtype=dtype, device=dev)
+        s = _like(x)
         sp = s.data_ptr()
     stats, mp = None, 0
     if keep:
-        stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+        stats = x.new_empty(2 * rows, dtype=torch.float32)
         mp = stats.data_ptr()
     x, xp, ldx, code = _rows(x, rows, D)
     z, zp, ldz, zcode = _rows(z, rows, D)
     w, wp, wcode = _vector(weight)
     b, bp, bcode = _vector(bias)
-    _fwd(dev, xp, zp, wp, bp, y.data_ptr(), sp, mp, mp and mp + 4 * rows, ldx, ldz, rows, D,
+    _fwd(x.device, xp, zp, wp, bp, y.data_ptr(), sp, mp, mp and mp + 4 * rows, ldx, ldz, rows, D,
          code, zcode, wcode, bcode, _CODE[y.dtype], eps)
     return y, s, stats
 
@@ -141,34 +147,33 @@ def _backward(ctx, s, weight, bias, dy, ds):
     dw, db), each None where it is not asked for."""
     D = math.prod(ctx.shape)
     rows = s.numel() // D
-    dev, dtype, shape = s.device, s.dtype, s.shape
+    dtype = s.dtype
     need_x, need_z, need_w, need_b = ctx.needs_input_grad[:4]
     d = dl = dw = db = part = None
     dp = lp = wgp = bgp = pp = lcode = 0
     if need_x or need_z:
-        d = torch.empty(shape, dtype=dtype, device=dev)
+        d = _like(s)
         dp = d.data_ptr()
         low = ctx.xdtype if ctx.xdtype != dtype else ctx.zdtype
         if low is not None and low != dtype:
-            dl = torch.empty(shape, dtype=low, device=dev)
+            dl = _like(s, low)
             lp, lcode = dl.data_ptr(), _CODE[low]
     w, wp, wcode = _vector(weight)
     if need_w:
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev)
+        dw = _like(weight)
         wgp = dw.data_ptr()
     if need_b:
-        db = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+        db = _like(bias)
         bgp = db.data_ptr()
     code = _CODE[dtype]
     if need_w or need_b:
-        part = torch.empty(_lib.lib().kfac_ln_ws_floats(code, rows, D), dtype=torch.float32,
-                           device=dev)
+        part = s.new_empty(_lib.lib().kfac_ln_ws_floats(code, rows, D), dtype=torch.float32)
         pp = part.data_ptr()
     s, sp, lds, _ = _rows(s, rows, D)
     g, gp, ldg, gcode = _rows(dy, rows, D)
     e, ep, lde, _ = _rows(ds, rows, D)
     mp = ctx.stats.data_ptr()
-    _bwd(dev, gp, ep, sp, wp, mp, mp + 4 * rows, dp, lp, wgp, bgp, pp, ldg, lde, lds, rows, D,
+    _bwd(s.device, gp, ep, sp, wp, mp, mp + 4 * rows, dp, lp, wgp, bgp, pp, ldg, lde, lds, rows, D,
          code, lcode, wcode, 0 if bias is None else _CODE[bias.dtype], gcode, 0)
     return d, dl, dw, db
 

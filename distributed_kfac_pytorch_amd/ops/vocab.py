@@ -156,7 +156,7 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.set_materialize_grads(False)
 
         def out(*more, dtype=dt):
-            return torch.empty(shape + more, dtype=dtype, device=dev)
+            return logits.new_empty(shape + more, dtype=dtype)
         lp = None if targets is None else out()
         h = out() if entropy else None
         tl, ti = (out(k), out(k, dtype=torch.int64)) if k else (None, None)
@@ -167,7 +167,7 @@ class _TokenLogprobs(torch.autograd.Function):
         elif _lib.use_native(logits):
             x, ld = _rows(logits, rows, V)
             code = _CODE[x.dtype]
-            stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
+            stats = logits.new_empty(2 * rows, dtype=torch.float32)
             ws, wp = _workspace(code, rows, V, k, dev)
             _fwd(dev, x.data_ptr(), _ptr(tgt), _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti),
                  stats.data_ptr(), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, 0, inv_t)
@@ -201,7 +201,7 @@ class _TokenLogprobs(torch.autograd.Function):
             return (None,) * 6
         V = logits.shape[-1]
         rows = logits.numel() // V
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dx = torch.empty_like(logits, memory_format=torch.contiguous_format)
         if rows == 0:
             return dx, None, None, None, None, None
         if _lib.use_native(logits):
@@ -284,15 +284,15 @@ class _TopkDistill(torch.autograd.Function):
         ids = ids.to(torch.int64).contiguous()
         teacher = teacher.contiguous()
         K = ids.shape[-1]
-        loss = torch.empty(logits.shape[:-1], dtype=dt, device=dev)
+        loss = logits.new_empty(logits.shape[:-1], dtype=dt)
         ctx.kept = None
         if rows and _lib.use_native(logits):
             x, ld = _rows(logits, rows, V)
             code = _CODE[x.dtype]
             # for the backward pass: (M, L) of the rows, each id once and its mass
-            stats = torch.empty(2 * rows, dtype=torch.float32, device=dev)
-            at = torch.empty(rows * K, dtype=torch.int32, device=dev)
-            mass = torch.empty(rows * K, dtype=torch.float32, device=dev)
+            stats = logits.new_empty(2 * rows, dtype=torch.float32)
+            at = ids.new_empty(rows * K, dtype=torch.int32)
+            mass = logits.new_empty(rows * K, dtype=torch.float32)
             ctx.kept = stats, at, mass
             ws, wp = _workspace(code, rows, V, 0, dev)
             _fwd(dev, x.data_ptr(), 0, 0, 0, 0, 0, stats.data_ptr(), ids.data_ptr(),
@@ -315,7 +315,7 @@ class _TopkDistill(torch.autograd.Function):
         logits, ids, teacher = ctx.saved_tensors
         V, K = logits.shape[-1], ids.shape[-1]
         rows = logits.numel() // V
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        dx = torch.empty_like(logits, memory_format=torch.contiguous_format)
         if rows and _lib.use_native(logits):
             x, ld = _rows(logits, rows, V)
             g, gp, gs = _row_grad(g)

@@ -36,7 +36,7 @@ struct KfacVocabFwd {
   const long long* targets;
   float *logprob, *entropy, *top_lp;
   long long* top_ids;
-  float* stats;                   // (M, L) a row
+  float* stats;                   // (M, L) a row, for the backward pass
   const long long* ids;           // teacher
   const void* teacher;
   float* loss;
@@ -569,9 +569,12 @@ __device__ __forceinline__ void distill_row(const Fwd& a, long long row, float M
   term = Group<NT>::sum(term, red);
   if (threadIdx.x == 0) {
     a.loss[row] = term;
-    a.stats[2 * row] = M;
-    a.stats[2 * row + 1] = z == z ? L : NAN;       // NaN all along the gradient's row
+    if (a.stats) {
+      a.stats[2 * row] = M;
+      a.stats[2 * row + 1] = z == z ? L : NAN;     // NaN all along the gradient's row
+    }
   }
+  if (!a.keep_ids) return;
   __syncthreads();
   // the same id twice: its masses are added in slot order, into its first slot
 #pragma unroll
@@ -616,8 +619,10 @@ __device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M
         t < 0 || t >= a.V ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[t]), M, L, a.inv_t);
   }
   if (a.entropy) a.entropy[row] = M == -INFINITY ? 0.f : L - sum / s * LN2;
-  a.stats[2 * row] = M;
-  a.stats[2 * row + 1] = L;
+  if (a.stats) {
+    a.stats[2 * row] = M;
+    a.stats[2 * row + 1] = L;
+  }
 }
 
 // (Six waves a SIMD also where both entropy and alternatives want registers:
@@ -645,8 +650,10 @@ void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
       if (a.loss) a.loss[row] = 0.f;
       if (a.logprob) a.logprob[row] = 0.f;
       if (a.entropy) a.entropy[row] = 0.f;
-      a.stats[2 * row] = -INFINITY;
-      a.stats[2 * row + 1] = 0.f;
+      if (a.stats) {
+        a.stats[2 * row] = -INFINITY;
+        a.stats[2 * row + 1] = 0.f;
+      }
     }
     return;
   }
@@ -906,15 +913,16 @@ KFAC_API long long kfac_vocab_ws_bytes(int dt, long long rows, long long V, int 
 
 // The argument record of ops/vocab.py (`bytes`: its size there).  Log
 // probabilities: targets null: no logprob; entropy null: none; k 0: no
-// alternatives.  Distillation: loss set, with ids, teacher, keep_ids, keep_q.
+// alternatives.  Distillation: loss set, with ids and teacher.  stats, and
+// keep_ids and keep_q of a distillation, null where no backward pass follows.
 KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t stream) {
   if (bytes != (int)sizeof(Fwd)) return -2;
   Fwd a = *args;
   if (!a.x || a.rows <= 0 || a.V <= 0 || a.V > MAX_V || a.rows > 0x7fffffffLL / MAX_SPLITS ||
-      !(a.inv_t > 0.f) || !dtype_ok(a.dt) || !a.stats)
+      !(a.inv_t > 0.f) || !dtype_ok(a.dt))
     return -2;
-  if (a.loss ? !a.ids || !a.teacher || !a.keep_ids || !a.keep_q || !dtype_ok(a.tdt) || a.K < 1 ||
-                   a.K > TOP_MAX || a.k
+  if (a.loss ? !a.ids || !a.teacher || !a.keep_ids != !a.keep_q || !a.keep_ids != !a.stats ||
+                   !dtype_ok(a.tdt) || a.K < 1 || a.K > TOP_MAX || a.k
              : a.k < 0 || a.k > TOP_MAX || a.k > a.V || (a.logprob && !a.targets) ||
                    (a.k && (!a.top_lp || !a.top_ids)))
     return -2;

@@ -144,53 +144,56 @@ def _cpu_entropy(lp, dead):
     return torch.where(dead, torch.zeros_like(h), h)
 
 
+def _logprobs(logits, targets, k, entropy, inv_t, ignore, keep):
+    """(logprobs, entropy, top_logprobs, top_ids, int64 targets, (M, L) where `keep`)."""
+    shape = logits.shape[:-1]
+    V = logits.shape[-1]
+    rows = logits.numel() // V
+    dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    lp = None if targets is None else logits.new_empty(shape, dtype=dt)
+    h = logits.new_empty(shape, dtype=dt) if entropy else None
+    tl = ti = stats = None
+    if k:
+        tl = logits.new_empty(shape + (k,), dtype=dt)
+        ti = logits.new_empty(shape + (k,), dtype=torch.int64)
+    tgt = None if targets is None else targets.to(torch.int64).contiguous()
+    if rows == 0:
+        pass
+    elif _lib.use_native(logits):
+        x, ld = _rows(logits, rows, V)
+        code = _CODE[x.dtype]
+        if keep:
+            stats = logits.new_empty(2 * rows, dtype=torch.float32)
+        ws, wp = _workspace(code, rows, V, k, logits.device)
+        _fwd(logits.device, x.data_ptr(), _ptr(tgt), _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti),
+             _ptr(stats), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, 0, inv_t)
+    else:
+        x, M, _, all_lp = _cpu_stats(logits.reshape(rows, V), inv_t)
+        skip = torch.zeros(rows, dtype=torch.bool) if tgt is None else tgt.reshape(-1) == ignore
+        if lp is not None:
+            v = _gather(all_lp, tgt.reshape(-1, 1).masked_fill(skip[:, None], 0))[:, 0]
+            lp.copy_(torch.where(skip, 0.0, v).view(shape))
+        if h is not None:
+            v = _cpu_entropy(all_lp, M == -math.inf)
+            h.copy_(torch.where(skip, 0.0, v).view(shape))
+        if k:
+            # stable, so that equal values keep the order of their indices
+            ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+            ti.copy_(ids.masked_fill(skip[:, None], -1).view(shape + (k,)))
+            tl.copy_(all_lp.gather(1, ids).masked_fill(skip[:, None], -math.inf)
+                     .view(shape + (k,)))
+    return lp, h, tl, ti, tgt, stats
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, k, entropy, inv_t, ignore):
-        shape = logits.shape[:-1]
-        V = logits.shape[-1]
-        rows = logits.numel() // V
-        dev = logits.device
-        dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
+        lp, h, tl, ti, tgt, ctx.stats = _logprobs(logits, targets, k, entropy, inv_t, ignore, True)
         ctx.inv_t, ctx.ignore = inv_t, ignore
         ctx.set_materialize_grads(False)
-
-        def out(*more, dtype=dt):
-            return logits.new_empty(shape + more, dtype=dtype)
-        lp = None if targets is None else out()
-        h = out() if entropy else None
-        tl, ti = (out(k), out(k, dtype=torch.int64)) if k else (None, None)
-        tgt = None if targets is None else targets.to(torch.int64).contiguous()
-        stats = None
-        if rows == 0:
-            pass
-        elif _lib.use_native(logits):
-            x, ld = _rows(logits, rows, V)
-            code = _CODE[x.dtype]
-            stats = logits.new_empty(2 * rows, dtype=torch.float32)
-            ws, wp = _workspace(code, rows, V, k, dev)
-            _fwd(dev, x.data_ptr(), _ptr(tgt), _ptr(lp), _ptr(h), _ptr(tl), _ptr(ti),
-                 stats.data_ptr(), 0, 0, 0, 0, 0, wp, ld, rows, V, ignore, code, k, 0, 0, 0, inv_t)
-        else:
-            x, M, L, all_lp = _cpu_stats(logits.reshape(rows, V), inv_t)
-            skip = torch.zeros(rows, dtype=torch.bool) if tgt is None else \
-                tgt.reshape(-1) == ignore
-            if lp is not None:
-                v = _gather(all_lp, tgt.reshape(-1, 1).masked_fill(skip[:, None], 0))[:, 0]
-                lp.copy_(torch.where(skip, 0.0, v).view(shape))
-            if h is not None:
-                v = _cpu_entropy(all_lp, M == -math.inf)
-                h.copy_(torch.where(skip, 0.0, v).view(shape))
-            if k:
-                # stable, so that equal values keep the order of their indices
-                ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
-                ti.copy_(ids.masked_fill(skip[:, None], -1).view(shape + (k,)))
-                tl.copy_(all_lp.gather(1, ids).masked_fill(skip[:, None], -math.inf)
-                         .view(shape + (k,)))
         if k:
             ctx.mark_non_differentiable(tl, ti)
         ctx.save_for_backward(logits, tgt, h)
-        ctx.stats = stats
         return lp, h, tl, ti
 
     @staticmethod
@@ -259,8 +262,10 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=False, temperature=1.0
     if targets is None and not k and not entropy:
         raise ValueError('token_logprobs: nothing asked for (no targets, top_k 0, no entropy)')
     _check_plain('token_logprobs', logits, targets)
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, targets, k, bool(entropy), inv_t,
-                                               int(ignore_index)))
+    args = logits, targets, k, bool(entropy), inv_t, int(ignore_index)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(*args))
+    return TokenLogprobs(*_logprobs(*args, False)[:4])
 
 
 def _cpu_teacher(ids, teacher, V, inv_t, dtype):
@@ -274,37 +279,42 @@ def _cpu_teacher(ids, teacher, V, inv_t, dtype):
     return some, ids.clamp(0, V - 1), d.exp() / Z, d - Z.log()
 
 
-class _TopkDistill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, inv_t):
-        V = logits.shape[-1]
-        rows = logits.numel() // V
-        dev = logits.device
-        dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
-        ids = ids.to(torch.int64).contiguous()
-        teacher = teacher.contiguous()
-        K = ids.shape[-1]
-        loss = logits.new_empty(logits.shape[:-1], dtype=dt)
-        ctx.kept = None
-        if rows and _lib.use_native(logits):
-            x, ld = _rows(logits, rows, V)
-            code = _CODE[x.dtype]
-            # for the backward pass: (M, L) of the rows, each id once and its mass
+def _distill(logits, ids, teacher, inv_t, keep):
+    """(losses, ids and teacher as they are read, what the GPU's backward pass
+    needs where `keep`: (M, L) of the rows, each id once and its mass)."""
+    V, K = logits.shape[-1], ids.shape[-1]
+    rows = logits.numel() // V
+    dt = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    ids = ids.to(torch.int64).contiguous()
+    teacher = teacher.contiguous()
+    loss = logits.new_empty(logits.shape[:-1], dtype=dt)
+    kept = None
+    if rows and _lib.use_native(logits):
+        x, ld = _rows(logits, rows, V)
+        code = _CODE[x.dtype]
+        stats = at = mass = None
+        if keep:
             stats = logits.new_empty(2 * rows, dtype=torch.float32)
             at = ids.new_empty(rows * K, dtype=torch.int32)
             mass = logits.new_empty(rows * K, dtype=torch.float32)
-            ctx.kept = stats, at, mass
-            ws, wp = _workspace(code, rows, V, 0, dev)
-            _fwd(dev, x.data_ptr(), 0, 0, 0, 0, 0, stats.data_ptr(), ids.data_ptr(),
-                 teacher.data_ptr(), loss.data_ptr(), at.data_ptr(), mass.data_ptr(), wp, ld, rows,
-                 V, 0, code, 0, K, _CODE[teacher.dtype], 0,
-                 inv_t)
-        elif rows:
-            lp = _cpu_stats(logits.reshape(rows, V), inv_t)[3]
-            some, at, q, logq = _cpu_teacher(ids.reshape(rows, K), teacher.reshape(rows, K), V,
-                                             inv_t, dt)
-            each = torch.where(q == 0, 0.0, q * (logq - lp.gather(1, at)))
-            loss.copy_(torch.where(some, each.sum(1), 0.0).view(loss.shape))
+            kept = stats, at, mass
+        ws, wp = _workspace(code, rows, V, 0, logits.device)
+        _fwd(logits.device, x.data_ptr(), 0, 0, 0, 0, 0, _ptr(stats), ids.data_ptr(),
+             teacher.data_ptr(), loss.data_ptr(), _ptr(at), _ptr(mass), wp, ld, rows, V, 0, code,
+             0, K, _CODE[teacher.dtype], 0, inv_t)
+    elif rows:
+        lp = _cpu_stats(logits.reshape(rows, V), inv_t)[3]
+        some, at, q, logq = _cpu_teacher(ids.reshape(rows, K), teacher.reshape(rows, K), V, inv_t,
+                                         dt)
+        each = torch.where(q == 0, 0.0, q * (logq - lp.gather(1, at)))
+        loss.copy_(torch.where(some, each.sum(1), 0.0).view(loss.shape))
+    return loss, ids, teacher, kept
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, inv_t):
+        loss, ids, teacher, ctx.kept = _distill(logits, ids, teacher, inv_t, True)
         ctx.save_for_backward(logits, ids, teacher)
         ctx.inv_t = inv_t
         return loss
@@ -377,4 +387,6 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
     if logits.is_cuda and teacher_logits.dtype == torch.float64:
         teacher_logits = teacher_logits.float()
     _check_plain(name, logits, teacher_ids, teacher_logits)
-    return _TopkDistill.apply(logits, teacher_ids, teacher_logits, inv_t)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TopkDistill.apply(logits, teacher_ids, teacher_logits, inv_t)
+    return _distill(logits, teacher_ids, teacher_logits, inv_t, False)[0]

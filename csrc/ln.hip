@@ -61,8 +61,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return r;
 }
 
-// Rows that no workgroup's registers hold (and rows shorter than one access):
-// the workgroup walks the row, once for each statistic and once for the
+// Rows that no workgroup's registers hold: the workgroup walks the row, once for each statistic and once for the
 // result; from the second time on it comes from a cache.
 
 // V elements at i, zeros from n on
@@ -228,7 +227,7 @@ __global__ __launch_bounds__(NT) void ln_param_part_kernel(const Bwd a) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows of V .. 16384 elements: a row is held in the registers of TR threads, E
+// Rows of up to 16384 elements: a row is held in the registers of TR threads, E
 // elements each in 16-byte accesses, so that x, z (forward) and dy, s, ds
 // (backward) are read once and the statistics are taken from registers.
 // Workgroups of 256 threads hold 256 / TR rows at a time (TR >= 256: one) and
@@ -260,12 +259,24 @@ template <int TR> struct RowSum {      // sums over the TR threads of a row
 
 // A thread's R accesses, issued back to back.  One that lies behind the row's
 // end for the whole wave is left out: a size class may be half empty.
-template <int DT, bool TAIL, bool STREAM, int R>
+// TINY: the row may be shorter than one access.
+template <int DT, bool TAIL, bool STREAM, bool TINY, int R>
 __device__ __forceinline__ void load_all(const AS1 typename DTypeTraits<DT>::raw_t* row, int t0,
                                          int step, int n, u32x4n* raw) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     raw[r] = (u32x4n)0u;
+    if constexpr (TINY) {
+      constexpr int V = row_vec<DT>();
+      if (n < V) {                       // the row's elements last, as clip_vec expects them
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          f[e] = t0 == 0 && r == 0 && e >= V - n ? DTypeTraits<DT>::to_f32(row[e - (V - n)]) : 0.f;
+        raw[r] = f32_to_vec<DT>(f);
+        continue;
+      }
+    }
     if (r == 0 || __builtin_amdgcn_readfirstlane(t0 + r * step) < n)
       raw[r] = load_vec<DT, TAIL, STREAM>(row, t0 + r * step, n);
   }
@@ -356,11 +367,11 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
       float g[E];
       // x and z are read for the last time: s is what the backward pass reads
       // (16384 x 4096 fp16: 104 -> 85 us)
-      load_all<DT, TAIL, true, R>(x, t0, step, D, raw);
+      load_all<DT, TAIL, true, TR == 16 && TAIL, R>(x, t0, step, D, raw);
       if (a.zdt == DT) {
         const AS1 raw_t* z = gptr((const raw_t*)a.z) + row * a.ldz;
         u32x4n zraw[R];
-        load_all<DT, TAIL, true, R>(z, t0, step, D, zraw);
+        load_all<DT, TAIL, true, TR == 16 && TAIL, R>(z, t0, step, D, zraw);
 #pragma unroll
         for (int r = 0; r < R; ++r)
           vec_to_f32<DT>(clip_vec<DT, TAIL>(zraw[r], t0 + r * step, D), g + r * V);
@@ -378,7 +389,7 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
         if (live) store_vec<DT, TAIL>(gptr((raw_t*)a.s) + row * D, i, D, f + r * V);
       }
     } else {
-      load_all<DT, TAIL, false, R>(x, t0, step, D, raw);
+      load_all<DT, TAIL, false, TR == 16 && TAIL, R>(x, t0, step, D, raw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(raw[r], t0 + r * step, D), f + r * V);
@@ -438,12 +449,12 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
     const AS1 raw_t* ds = gptr((const raw_t*)a.ds) + row * a.ldds;
     float h[E], g[E];
     u32x4n sraw[R], eraw[R];
-    load_all<DT, TAIL, true, R>(s, t0, step, D, sraw);
-    if (a.ds) load_all<DT, TAIL, true, R>(ds, t0, step, D, eraw);
+    load_all<DT, TAIL, true, TR == 16 && TAIL, R>(s, t0, step, D, sraw);
+    if (a.ds) load_all<DT, TAIL, true, TR == 16 && TAIL, R>(ds, t0, step, D, eraw);
     if (a.ydt == DT) {
       const AS1 raw_t* dy = gptr((const raw_t*)a.dy) + row * a.lddy;
       u32x4n graw[R];
-      load_all<DT, TAIL, true, R>(dy, t0, step, D, graw);
+      load_all<DT, TAIL, true, TR == 16 && TAIL, R>(dy, t0, step, D, graw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(graw[r], t0 + r * step, D), g + r * V);
@@ -548,7 +559,7 @@ constexpr long long LONG_ROW = 16384;     // longer rows: the kernels that loop 
 
 #define LN_SIZES(F) F(16, 8) F(32, 8) F(64, 8) F(64, 16) F(128, 16) F(256, 16) F(512, 16) F(1024, 16)
 
-bool looped(int dt, long long D) { return D > LONG_ROW || D < (dt == KDT_F32 ? 4 : 8); }
+bool looped(long long D) { return D > LONG_ROW; }
 
 // threads a row
 int row_threads(long long D) {
@@ -574,8 +585,8 @@ constexpr long long FWD_BLOCKS = 4096;
 // need 1024, a workgroup for every CU (8192 x 16384 fp16 342 | 224).
 long long bwd_blocks(long long D) { return D > 512 && D <= 8192 ? 512 : 1024; }
 
-int param_chunks(int dt, long long rows, long long D) {
-  if (!looped(dt, D)) return (int)row_blocks(rows, D, bwd_blocks(D));
+int param_chunks(long long rows, long long D) {
+  if (!looped(D)) return (int)row_blocks(rows, D, bwd_blocks(D));
   const long long c = (rows + 63) / 64;
   return (int)(c < 512 ? c : 512);
 }
@@ -597,7 +608,7 @@ void launch_bwd(const Bwd& a, hipStream_t st) {
     hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, false>), grid, block, 0, st, a);
 }
 template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
-  if (looped(DT, a.D)) {
+  if (looped(a.D)) {
     hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
     return;
   }
@@ -608,7 +619,7 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
 #undef F
 }
 template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
-  if (looped(DT, a.D)) {
+  if (looped(a.D)) {
     if (a.dx)
       hipLaunchKernelGGL(ln_bwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
     const long long cols = NT * row_vec<DT>();
@@ -627,8 +638,8 @@ template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
 }  // namespace
 
 // floats of the workspace of one backward call that asks for dw or db
-KFAC_API long long kfac_ln_ws_floats(int sdt, long long rows, long long D) {
-  return 2LL * param_chunks(sdt, rows, D) * D;
+KFAC_API long long kfac_ln_ws_floats(long long rows, long long D) {
+  return 2LL * param_chunks(rows, D) * D;
 }
 
 // The argument record of ops/ln.py (`bytes`: its size there).  z and s null:
@@ -658,7 +669,7 @@ KFAC_API int kfac_ln_backward(const KfacLnBwd* args, int bytes, hipStream_t stre
       ((a.dw || a.db) && !a.part))
     return -2;
   if (!a.dw && !a.db) a.part = nullptr;
-  a.chunks = param_chunks(a.sdt, a.rows, a.D);
+  a.chunks = param_chunks(a.rows, a.D);
   if (a.sdt == KDT_F32) launch_bwd_any<KDT_F32>(a, stream);
   else if (a.sdt == KDT_BF16) launch_bwd_any<KDT_BF16>(a, stream);
   else launch_bwd_any<KDT_F16>(a, stream);

@@ -153,7 +153,7 @@ _SIGS = {
     'kfac_dc_ws_bytes': [c_int],
     'kfac_dc_set_fast_scan': [c_int],
     'kfac_dc_info_offset': [c_int],
-    'kfac_ln_ws_floats': [c_int, c_ll, c_ll],
+    'kfac_ln_ws_floats': [c_ll, c_ll],
     'kfac_ln_forward': [ctypes.c_char_p, c_int, c_vp],
     'kfac_ln_backward': [ctypes.c_char_p, c_int, c_vp],
     'kfac_vocab_top_max': [],
@@ -255,11 +255,12 @@ class PackedCall(object):
 
 
 def plain_tensors(*tensors):
-    """True where raw pointers may be taken: ordinary tensors, and neither a
-    functorch transform, a forward-mode level nor a compile trace around them
-    (each of these needs torch operations that it knows)."""
-    if torch.compiler.is_compiling() or torch._C._are_functorch_transforms_active() \
-            or forward_ad._current_level >= 0:
+    """True where raw pointers may be taken: ordinary tensors, and no functorch
+    transform, forward-mode level, dispatch mode or trace around them (each of
+    these needs torch operations that it can see)."""
+    if torch.compiler.is_compiling() or torch._C._is_tracing() \
+            or torch._C._len_torch_dispatch_stack() \
+            or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
         return False
     return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter
                for t in tensors)

@@ -12,7 +12,7 @@ type of s (fp32 under autocast, which runs layer norms in fp32).  On a GPU, for
 fp32 / bf16 / fp16 tensors, it is one kernel forward and two or three backward
 (hipGraph-capturable, bitwise reproducible; statistics and all sums in fp32);
 anything else (CPU tensors, fp64, tensor subclasses, z of another shape,
-functorch transforms, torch.compile traces) takes the two torch operations.
+functorch transforms, dispatch modes, traces) takes the two torch operations.
 Unlike F.layer_norm, the weights may have another type than x.
 `KFAC_FUSED_LN=0` disables the kernels.
 
@@ -44,7 +44,8 @@ def eligible(x, normalized_shape, weight=None, bias=None, z=None):
     if not (ENABLED and x.is_cuda and x.dtype in _CODE and x.numel() > 0):
         return False
     n = len(normalized_shape)
-    if n == 0 or x.shape[-n:] != normalized_shape:
+    if n == 0 or x.shape[-n:] != normalized_shape or \
+            x.numel() // math.prod(normalized_shape) >= 2 ** 31:
         return False
     if z is not None and (z.shape != x.shape or z.dtype not in _CODE or z.device != x.device):
         return False
@@ -167,7 +168,7 @@ def _backward(ctx, s, weight, bias, dy, ds):
         bgp = db.data_ptr()
     code = _CODE[dtype]
     if need_w or need_b:
-        part = s.new_empty(_lib.lib().kfac_ln_ws_floats(code, rows, D), dtype=torch.float32)
+        part = s.new_empty(_lib.lib().kfac_ln_ws_floats(rows, D), dtype=torch.float32)
         pp = part.data_ptr()
     s, sp, lds, _ = _rows(s, rows, D)
     g, gp, ldg, gcode = _rows(dy, rows, D)

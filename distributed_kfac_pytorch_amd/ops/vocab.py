@@ -81,7 +81,7 @@ def _check_ids(name, what, t, shape, device):
 def _check_plain(name, *tensors):
     if not _lib.plain_tensors(*tensors):
         raise TypeError('{}: takes ordinary tensors, outside functorch transforms, forward-mode '
-                        'levels and compile traces'.format(name))
+                        'levels, dispatch modes and traces'.format(name))
 
 
 def _rows(t, rows, V):

@@ -77,7 +77,7 @@ def check(name, got, want):
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (1, 512), (4, 511), (33, 513), (700, 650), (9, 1024),
           (2, 3, 2049), (5, 4097), (3, 8192), (2, 12289), (2, 16384), (2, 16387), (1, 70001),
-          (1031, 24), (5000, 40), (2100, 1032)]
+          (1031, 24), (5000, 40), (2100, 1032), (300, 1), (300, 3), (99, 4), (99, 5), (77, 8), (77, 9)]
 TYPES = [(F32, None), (BF16, None), (F16, None), (F32, F32), (BF16, BF16), (F16, F16)]
 MIXED = [(F32, BF16), (BF16, F32), (F16, F32), (BF16, F16)]
 
@@ -313,6 +313,43 @@ def test_bitwise_repeatable_and_captured(rows, D, dtype):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, ref)), k
+
+
+@pytest.mark.parametrize('D', [64, 20000])
+def test_offsets_past_32_bits(D):
+    """The last rows of more than 2^31 elements, 2^32 bytes."""
+    rows = 2 ** 31 // D + 5
+    x = torch.zeros(rows, D, dtype=BF16, device=DEV)
+    x[-3:] = make((3, D), BF16)
+    x.requires_grad_(True)
+    w = make((D,), BF16, 2).requires_grad_(True)
+    y = ln.layer_norm(x, D, w)
+    dy = torch.zeros_like(y)
+    dy[-3:] = make((3, D), BF16, 3)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    o = oracle(x.detach()[-3:], w, None, 1e-5, dy[-3:])
+    check('y', y[-3:], o['y'])
+    check('dx', dx[-3:], o['dx'])
+    check('dw', dw, o['dw'])
+    assert not y[:-3].any() and not dx[:-3].any()
+
+
+def test_traces_and_modes_see_torch():
+    """A trace of the module and a dispatch mode around it hold torch's own norm."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    m = LayerNorm(32, device=DEV)
+    x, x2 = make((4, 32), F32), make((4, 32), F32, 2)
+    t = torch.jit.trace(m, (x,))
+    check('trace', t(x2), oracle(x2, None, None, 1e-5)['y'])
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Mode():
+        m(x)
+    assert any('layer_norm' in s for s in seen)
 
 
 def test_module_switch(monkeypatch):

@@ -366,6 +366,48 @@ def test_refusals_on_the_gpu():
     assert _lib.lib().kfac_vocab_top_max() == vocab.TOP_MAX
 
 
+def test_no_rows_on_the_gpu():
+    x = torch.empty(0, 5, device=DEV, requires_grad=True)
+    r = vocab.token_logprobs(x, torch.empty(0, dtype=torch.long, device=DEV), top_k=2,
+                             entropy=True)
+    loss = vocab.topk_distill_loss(x, torch.empty(0, 3, dtype=torch.long, device=DEV),
+                                   torch.empty(0, 3, device=DEV))
+    g, = torch.autograd.grad((r.logprobs + r.entropy + loss).sum(), x)
+    assert g.shape == (0, 5) and r.top_ids.shape == (0, 2)
+
+
+def test_without_a_graph_the_same_values():
+    x = logits(9, 2003, BF16)
+    t = torch.randint(0, 2003, (9,), device=DEV)
+    ids, q = teacher(9, 2003, 7, F32)
+    a = vocab.token_logprobs(x, t, top_k=3, entropy=True)
+    la = vocab.topk_distill_loss(x, ids, q)
+    x.requires_grad_(True)
+    b = vocab.token_logprobs(x, t, top_k=3, entropy=True)
+    lb = vocab.topk_distill_loss(x, ids, q)
+    assert b.logprobs.requires_grad and lb.requires_grad and not la.requires_grad
+    assert all(torch.equal(u, v) for u, v in zip(a, b)) and torch.equal(la, lb)
+
+
+def test_checkpointed_and_repeated_backward():
+    """Recomputed in a checkpoint, and twice from one graph: the same gradient."""
+    from torch.utils.checkpoint import checkpoint
+    head = torch.nn.Linear(16, 700, device=DEV)
+    h = torch.randn(6, 16, device=DEV)
+    t = torch.randint(0, 700, (6,), device=DEV)
+    ids, q = teacher(6, 700, 5, F32)
+
+    def f(h):
+        x = head(h)
+        r = vocab.token_logprobs(x, t, entropy=True)
+        return (vocab.topk_distill_loss(x, ids, q) - r.logprobs - 0.1 * r.entropy).sum()
+    loss = f(h)
+    a = torch.autograd.grad(loss, head.weight, retain_graph=True)[0]
+    b = torch.autograd.grad(loss, head.weight)[0]
+    c = torch.autograd.grad(checkpoint(f, h, use_reentrant=False), head.weight)[0]
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
 def test_runs_in_fp16_training():
     """Autocast and a scaled loss: fp16 logits, gradients in fp16."""
     head = torch.nn.Linear(32, 500).to(DEV)

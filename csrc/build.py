@@ -1,12 +1,14 @@
-"""Build the gfx950 HIP kernel library in-tree.
+"""Build the gfx950 HIP kernel library and its torch operators in-tree.
 
     python csrc/build.py [--force] [--jobs N]
 
 Compiles every csrc/*.hip with `hipcc --offload-arch=gfx950` into object
 files under build/, links them into
 `distributed_kfac_pytorch_amd/_native/libkfac_hip.so` (plain C ABI, loaded
-through ctypes by ops/_lib.py; no torch headers, no hipify).  Rebuilds only
-when a source or header is newer than the library.
+through ctypes by ops/_lib.py; no torch headers, no hipify).  csrc/torch_ops.cpp
+(host code only: autograd nodes over the C ABI) becomes
+`_native/libkfac_torch.so` with the host compiler and torch's headers.  Rebuilds
+only when a source or header is newer than the library.
 """
 import argparse
 import concurrent.futures
@@ -19,6 +21,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, 'csrc')
 OUT_DIR = os.path.join(ROOT, 'distributed_kfac_pytorch_amd', '_native')
 LIB = os.path.join(OUT_DIR, 'libkfac_hip.so')
+TORCH_LIB = os.path.join(OUT_DIR, 'libkfac_torch.so')
 BUILD = os.path.join(ROOT, 'build', 'hip')
 ARCH = os.environ.get('KFAC_HIP_ARCH', 'gfx950')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
@@ -77,7 +80,38 @@ def compile_optional():
     return [_compile(os.path.join(CSRC, f)) for f in TWO_STAGE_SOURCES]
 
 
+def build_torch_ops(force=False, verbose=True):
+    src = os.path.join(CSRC, 'torch_ops.cpp')
+    deps = [src, os.path.join(CSRC, 'records.h')]
+    if not force and not _stale(TORCH_LIB, deps):
+        return TORCH_LIB
+    import torch
+    from torch.utils import cpp_extension
+    rocm = os.path.dirname(os.path.dirname(HIPCC)) if os.path.isabs(HIPCC) else '/opt/rocm'
+    tmp = TORCH_LIB + '.tmp'
+    cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared',
+           '-D__HIP_PLATFORM_AMD__=1',                 # the HIP headers behind torch's streams
+           '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for d in cpp_extension.include_paths() + [os.path.join(rocm, 'include')]:
+        cmd += ['-isystem', d]
+    cmd += ['-I', CSRC, src, '-o', tmp, '-L', OUT_DIR, '-lkfac_hip', '-Wl,-rpath,$ORIGIN',
+            '-L', cpp_extension.TORCH_LIB_PATH, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch']
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError('host compiler failed:\n{}\n{}'.format(' '.join(cmd), r.stderr))
+    os.replace(tmp, TORCH_LIB)
+    if verbose:
+        print('built', TORCH_LIB)
+    return TORCH_LIB
+
+
 def build(force=False, jobs=None, verbose=True):
+    lib = build_kernels(force, jobs, verbose)
+    build_torch_ops(force, verbose)
+    return lib
+
+
+def build_kernels(force=False, jobs=None, verbose=True):
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sources()

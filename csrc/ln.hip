@@ -12,26 +12,8 @@
 // sum are held in fp32, the variance about the mean (two passes over the row).
 // The sums over rows (dw, db) run over fixed row chunks and then over the
 // chunks in order: no atomics, bitwise reproducible.
+#include "records.h"
 #include "rows.h"
-
-// argument records (ops/ln.py packs the same fields); chunks is set here
-struct KfacLnFwd {
-  const void *x, *z, *w, *b;
-  void *y, *s;
-  float *mean, *rstd;
-  long long ldx, ldz, rows, D;
-  int sdt, zdt, wdt, bdt, ydt;
-  float eps;
-};
-
-struct KfacLnBwd {
-  const void *dy, *ds, *s, *w;
-  const float *mean, *rstd;
-  void *dx, *dz, *dw, *db;
-  float* part;
-  long long lddy, ldds, lds, rows, D;
-  int sdt, zdt, wdt, bdt, ydt, chunks;
-};
 
 namespace {
 
@@ -642,11 +624,7 @@ KFAC_API long long kfac_ln_ws_floats(long long rows, long long D) {
   return 2LL * param_chunks(rows, D) * D;
 }
 
-// The argument record of ops/ln.py (`bytes`: its size there).  z and s null:
-// the norm of x.  w, b may be null; mean, rstd (fp32, one a row) may be null
-// where no backward pass follows.
-KFAC_API int kfac_ln_forward(const KfacLnFwd* args, int bytes, hipStream_t stream) {
-  if (bytes != (int)sizeof(KfacLnFwd)) return -2;
+KFAC_API int kfac_ln_forward(const KfacLnFwd* args, hipStream_t stream) {
   const Fwd a = *args;
   if (!a.x || !a.y || a.rows <= 0 || a.rows > 0x7fffffffLL || a.D <= 0 || !dtype_ok(a.sdt) ||
       !dtype_ok(a.ydt) || (a.z && (!a.s || !dtype_ok(a.zdt))) || (a.w && !dtype_ok(a.wdt)) ||
@@ -658,10 +636,7 @@ KFAC_API int kfac_ln_forward(const KfacLnFwd* args, int bytes, hipStream_t strea
   return (int)hipGetLastError();
 }
 
-// ds (the gradient that reaches s itself), dx, dz, dw, db may be null; part
-// (kfac_ln_ws_floats) is needed where dw or db is asked for
-KFAC_API int kfac_ln_backward(const KfacLnBwd* args, int bytes, hipStream_t stream) {
-  if (bytes != (int)sizeof(KfacLnBwd)) return -2;
+KFAC_API int kfac_ln_backward(const KfacLnBwd* args, hipStream_t stream) {
   Bwd a = *args;
   if (!a.dy || !a.s || !a.mean || !a.rstd || a.rows <= 0 || a.rows > 0x7fffffffLL || a.D <= 0 ||
       !dtype_ok(a.sdt) || !dtype_ok(a.ydt) || (a.dz && (!a.dx || !dtype_ok(a.zdt))) ||

@@ -28,38 +28,8 @@
 // gradient; NaN or +inf in a row, or a target out of range, makes its results
 // NaN; a teacher row without a used slot (id -1) or with only -inf gives
 // loss 0 and no gradient.
+#include "records.h"
 #include "rows.h"
-
-// argument records (ops/vocab.py packs the same fields)
-struct KfacVocabFwd {
-  const void* x;
-  const long long* targets;
-  float *logprob, *entropy, *top_lp;
-  long long* top_ids;
-  float* stats;                   // (M, L) a row, for the backward pass
-  const long long* ids;           // teacher
-  const void* teacher;
-  float* loss;
-  int* keep_ids;                  // ids (each once) and masses for the backward pass
-  float* keep_q;
-  void* ws;
-  long long ld, rows, V, ignore;
-  int dt, k, K, tdt, stream;
-  float inv_t;
-};
-
-struct KfacVocabBwd {
-  const void* x;
-  const float *stats, *entropy;
-  const long long* targets;
-  const float *g, *gh;
-  const int* keep_ids;
-  const float* keep_q;
-  void* dx;
-  long long ld, rows, V, ignore, gs, ghs;
-  int dt, K;
-  float inv_t;
-};
 
 namespace {
 
@@ -911,12 +881,7 @@ KFAC_API long long kfac_vocab_ws_bytes(int dt, long long rows, long long V, int 
   return splits == 1 ? 0 : rows * splits * (long long)(sizeof(Part) + 8LL * k);
 }
 
-// The argument record of ops/vocab.py (`bytes`: its size there).  Log
-// probabilities: targets null: no logprob; entropy null: none; k 0: no
-// alternatives.  Distillation: loss set, with ids and teacher.  stats, and
-// keep_ids and keep_q of a distillation, null where no backward pass follows.
-KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t stream) {
-  if (bytes != (int)sizeof(Fwd)) return -2;
+KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, hipStream_t stream) {
   Fwd a = *args;
   if (!a.x || a.rows <= 0 || a.V <= 0 || a.V > MAX_V || a.rows > 0x7fffffffLL / MAX_SPLITS ||
       !(a.inv_t > 0.f) || !dtype_ok(a.dt))
@@ -934,11 +899,7 @@ KFAC_API int kfac_vocab_forward(const KfacVocabFwd* args, int bytes, hipStream_t
   return (int)hipGetLastError();
 }
 
-// g, gh: gradients of logprob (or of the loss) and of the entropy, one a row at
-// a distance of gs, ghs elements (0: the same for every row); gh, and g of log
-// probabilities, may be null
-KFAC_API int kfac_vocab_backward(const KfacVocabBwd* args, int bytes, hipStream_t stream) {
-  if (bytes != (int)sizeof(Bwd)) return -2;
+KFAC_API int kfac_vocab_backward(const KfacVocabBwd* args, hipStream_t stream) {
   const Bwd a = *args;
   if (!a.x || !a.dx || !a.stats || a.rows <= 0 || a.V <= 0 || a.V > MAX_V ||
       a.rows > 0x7fffffffLL / ((a.V + 4095) / 4096) || !(a.inv_t > 0.f) || !dtype_ok(a.dt))

@@ -9,7 +9,6 @@ used only for CPU tensors).
 """
 import ctypes
 import os
-import struct
 import threading
 
 import torch
@@ -17,10 +16,12 @@ from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_HERE, '_native', 'libkfac_hip.so')
+TORCH_LIB_PATH = os.path.join(_HERE, '_native', 'libkfac_torch.so')
 
 _lock = threading.Lock()
 _lib = None
 _load_error = None
+_torch_ops = None
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 
@@ -153,13 +154,7 @@ _SIGS = {
     'kfac_dc_ws_bytes': [c_int],
     'kfac_dc_set_fast_scan': [c_int],
     'kfac_dc_info_offset': [c_int],
-    'kfac_ln_ws_floats': [c_ll, c_ll],
-    'kfac_ln_forward': [ctypes.c_char_p, c_int, c_vp],
-    'kfac_ln_backward': [ctypes.c_char_p, c_int, c_vp],
     'kfac_vocab_top_max': [],
-    'kfac_vocab_ws_bytes': [c_int, c_ll, c_ll, c_int],
-    'kfac_vocab_forward': [ctypes.c_char_p, c_int, c_vp],
-    'kfac_vocab_backward': [ctypes.c_char_p, c_int, c_vp],
     'kfac_bn_ws_floats': [c_ll, c_int],
     'kfac_bn_forward': [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_ll,
                         c_int, ctypes.c_float, ctypes.c_float, c_int, c_vp],
@@ -172,8 +167,7 @@ _RESTYPES = {'kfac_dc_ws_bytes': c_ll, 'kfac_sy2sb_ws_floats': c_ll,
              'kfac_reduce_ws_floats': c_ll, 'kfac_syrk_splits': c_ll,
              'kfac_chol_ws_bytes': c_ll, 'kfac_chol_info_offset': c_ll,
              'kfac_syrk_problem_set_part': None, 'kfac_syrk_problem_set_dscale': None,
-             'kfac_bn_ws_floats': c_ll, 'kfac_ln_ws_floats': c_ll, 'kfac_vocab_ws_bytes': c_ll,
-             'kfac_event_create': c_vp}
+             'kfac_bn_ws_floats': c_ll, 'kfac_event_create': c_vp}
 
 
 def _load():
@@ -231,27 +225,18 @@ def use_native(t):
     return True
 
 
-class PackedCall(object):
-    """A C entry point `int name(const Record*, int bytes, hipStream_t)`, called
-    with the record's fields: they are packed by one struct format (pack and call:
-    0.3 us) and launched on the current stream of `device`, with `device` current
-    (a launch goes to the current device, also where its tensors belong to another)."""
-
-    def __init__(self, name, fmt):
-        self.name, self.size = name, struct.calcsize(fmt)
-        self.pack = struct.Struct(fmt).pack
-
-    def __call__(self, device, *fields):
-        index = device.index
-        fn = getattr(lib(), self.name)
-        if index == torch._C._cuda_getDevice():
-            err = fn(self.pack(*fields), self.size, torch._C._cuda_getCurrentRawStream(index))
-        else:
-            with torch.cuda.device(index):
-                err = fn(self.pack(*fields), self.size,
-                         torch._C._cuda_getCurrentRawStream(index))
-        if err:
-            check(err, self.name)
+def torch_ops():
+    """torch.ops.kfac_hip: the operators of csrc/torch_ops.cpp (autograd nodes in
+    C++ over the same library); raises (never falls back) when it is missing."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib()
+        if not os.path.exists(TORCH_LIB_PATH):
+            raise RuntimeError('distributed_kfac_pytorch_amd torch operators not built: {} '
+                               '(run `python csrc/build.py`)'.format(TORCH_LIB_PATH))
+        torch.ops.load_library(TORCH_LIB_PATH)
+        _torch_ops = torch.ops.kfac_hip
+    return _torch_ops
 
 
 def plain_tensors(*tensors):

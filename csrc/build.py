@@ -85,8 +85,12 @@ def build_torch_ops(force=False, verbose=True):
     deps = [src, os.path.join(CSRC, 'records.h')]
     if not force and not _stale(TORCH_LIB, deps):
         return TORCH_LIB
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError:           # an isolated build: the operators on GPU tensors will say so
+        print('torch not found: the kernels are built, their torch operators are not')
+        return None
     rocm = os.path.dirname(os.path.dirname(HIPCC)) if os.path.isabs(HIPCC) else '/opt/rocm'
     tmp = TORCH_LIB + '.tmp'
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared',

@@ -18,10 +18,13 @@
 // brought to a new maximum once per tile of 16 elements; the threads'
 // (m, s, a) are joined at the end.  The alternatives need no second pass: the
 // k-th largest of the threads' maxima is a bound that at least k elements
-// reach, and only the threads that reach it have such elements, so about k of
-// 256 threads' elements are looked at again.  A row is cut over several
+// reach, and of the threads that reach it only the runs of tiles whose maximum
+// does are looked at again: about k of 2048.  A row is cut over several
 // workgroups where there are few rows, and joined by a second kernel.
 // Backward: one read and one write of the row from the saved (M, L).
+//
+// Both are bound by HBM: 4 to 8 instructions and one exponential an element are
+// about 60 % of the time that a 16-bit element takes to arrive.
 //
 // Defined edges: a row whose target is `ignore` is neither read nor gives a
 // gradient (0, ids -1); a row of only -inf has logprob -inf, entropy 0 and no
@@ -35,7 +38,6 @@ namespace {
 
 typedef KfacVocabFwd Fwd;
 typedef KfacVocabBwd Bwd;
-
 
 constexpr int TOP_MAX = 128;      // alternatives, and slots of a teacher's row
 constexpr int MAX_V = 1 << 30;    // elements of a row: 32-bit offsets within it
@@ -608,6 +610,10 @@ __device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M
   }
 }
 
+// One workgroup a chunk of a row.  4096 x 131072 bf16 160 us (6.7 TB/s), 2048 x
+// 32064 fp32 with entropy 43 us (6.1 TB/s), 8192 x 50001 bf16 with entropy and 32
+// alternatives 165 us (5.0 TB/s; 131 us without either), 700 x 10000 fp32 with 5 of
+// them 12.5 us; one row of 131072 8 us, where the round trips to memory count.
 // (Six waves a SIMD also where both entropy and alternatives want registers:
 // 8192 x 50001 bf16 with 32 of them 189 -> 177 us.  Without either it costs.)
 template <int DT, int NT, int MODE, bool ENT, bool TOP>
@@ -676,7 +682,8 @@ void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
   }
 }
 
-// Joins the parts of a row.  The alternatives: every part has its own k largest
+// Joins the parts of a row (one of 131072 in 32 parts, 20 alternatives: 5.6 us, the
+// launch and four dependent loads).  The alternatives: every part has its own k largest
 // in order; with j of a part's keys at least as large as the r-th largest of
 // all parts' j-th keys, r j >= k, that key is a bound which at least k keys
 // reach and no more than r k + splits j.
@@ -751,11 +758,13 @@ __global__ __launch_bounds__(JOIN_NT) void vocab_join_kernel(const Fwd a, int sp
   }
 }
 
-// One workgroup writes BWD_TILES tiles of four 16-byte accesses a thread, then
-// corrects the few elements that carry the target's or the teacher's mass.
-constexpr int BWD_NT = 256, BWD_TILES = 1;
+// One workgroup writes one tile of four 16-byte accesses a thread, then corrects
+// the few elements that carry the target's or the teacher's mass.  A read and a
+// write of every element: 4096 x 131072 bf16 355 us (6.1 TB/s; one access a thread
+// in a bare copy reaches 6.2), 2048 x 32064 fp32 84 us (5.9 TB/s).
+constexpr int BWD_NT = 256;
 
-template <int DT> constexpr int bwd_chunk() { return BWD_NT * row_vec<DT>() * 4 * BWD_TILES; }
+template <int DT> constexpr int bwd_chunk() { return BWD_NT * row_vec<DT>() * 4; }
 
 template <int DT, int MODE, bool ENT>
 __global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int splits) {

@@ -147,6 +147,14 @@ def test_rows_of_hard_values(kind, dtype):
     run_case((7, 650), dtype, None, make_=rows)
 
 
+def test_a_constant_row_is_its_bias():
+    """The mean of equal values is that value (sums of up to 2^24 units are exact)."""
+    for D in (3, 512, 650, 4097, 20000):
+        b = make((D,), F32, 2)
+        y = ln.layer_norm(torch.full((4, D), 3.0, device=DEV), D, make((D,), F32, 3), b)
+        assert torch.equal(y, b.expand(4, D))
+
+
 def test_a_bad_row_stays_its_own():
     x = make((6, 130), F32)
     ref = ln.layer_norm(x, 130)

@@ -408,6 +408,39 @@ def test_checkpointed_and_repeated_backward():
     assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_second_derivatives_are_errors():
+    x = logits(2, 50, F32).requires_grad_(True)
+    r = vocab.token_logprobs(x, torch.tensor([1, 2], device=DEV), entropy=True)
+    loss = vocab.topk_distill_loss(x, torch.tensor([[1], [2]], device=DEV), x.detach()[:, :1])
+    for out in (r.logprobs, r.entropy, loss):
+        g, = torch.autograd.grad(out.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
+def test_saved_inputs_are_guarded():
+    """Logits or targets written over before the backward pass are an error; a
+    teacher written over changes nothing (its masses were kept)."""
+    t = torch.tensor([1, 2], device=DEV)
+    base = logits(2, 50, F32).requires_grad_(True)
+    x = base * 1
+    lp = vocab.token_logprobs(x, t).logprobs
+    t.add_(1)
+    with pytest.raises(RuntimeError):
+        lp.sum().backward()
+    lp = vocab.token_logprobs(x, t).logprobs
+    x.detach().mul_(2)
+    with pytest.raises(RuntimeError):
+        lp.sum().backward()
+    x = base * 1
+    ids, q = teacher(2, 50, 4, F32)
+    o = oracle.distill(x.detach(), ids, q, g=torch.ones(2))
+    loss = vocab.topk_distill_loss(x, ids, q)
+    ids.fill_(-1)
+    q.zero_()
+    oracle.check('dlogits', torch.autograd.grad(loss.sum(), x)[0], o['dlogits'])
+
+
 def test_runs_in_fp16_training():
     """Autocast and a scaled loss: fp16 logits, gradients in fp16."""
     head = torch.nn.Linear(32, 500).to(DEV)

@@ -44,14 +44,18 @@ inline const void* get(const void* host, size_t bytes, hipStream_t stream, int* 
   auto it = c.map.find(key);
   if (it != c.map.end()) return it->second;
   const size_t need = (bytes + 255) / 256 * 256;
-  if (c.used + need > c.cap) {
-    // a new arena (allocation is not capturable: the first use of a table
-    // happens in an eager warm-up run in practice)
-    const size_t cap = need > (size_t)(4 << 20) ? need : (size_t)(4 << 20);
+  // A new arena cannot be allocated inside a capture, so an eager call begins one
+  // while the old one still has room for what a capture may bring (a training
+  // step's tables: some 100 KB).
+  const size_t reserve = (size_t)1 << 20;
+  hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+  const bool capturing = hipStreamIsCapturing(stream, &cs) == hipSuccess &&
+                         cs != hipStreamCaptureStatusNone;
+  if (c.used + need + (capturing ? 0 : reserve) > c.cap) {
+    const size_t cap = need + reserve > (size_t)(4 << 20) ? need + reserve : (size_t)(4 << 20);
     char* d = nullptr;
     char* h = nullptr;
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone) {
+    if (capturing) {
       *err = -20;   // would allocate inside a capture
       return nullptr;
     }

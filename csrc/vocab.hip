@@ -543,8 +543,11 @@ __device__ __forceinline__ void distill_row(const Fwd& a, long long row, float M
     q[p] = __builtin_amdgcn_exp2f(d * LOG2E) / z;
     const int j = threadIdx.x + p * NT;
     if (j < a.K && q[p] != 0.f) {
-      const float lp = id[p] < 0 ? NAN : log_prob(DTypeTraits<DT>::to_f32(x[id[p]]), M, L, a.inv_t);
-      term += q[p] * (d - logz - lp);
+      // q (log q - lp) with q taken into lp's product first: of a token masked by the
+      // type's lowest value (x - M) / T is past fp32's range, and q may be nothing
+      const float c = id[p] < 0 ? NAN : M == -INFINITY ? -INFINITY
+                                      : DTypeTraits<DT>::to_f32(x[id[p]]) - M;
+      term += q[p] * (d - logz + (M == -INFINITY ? 0.f : L)) - q[p] * c * a.inv_t;
     }
     if (j < TOP_MAX) {
       sh.id[j] = id[p];

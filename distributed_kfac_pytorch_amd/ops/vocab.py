@@ -200,12 +200,16 @@ class _TopkDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, inv_t):
         V, K = logits.shape[-1], ids.shape[-1]
-        lp = _cpu_stats(logits.reshape(-1, V), inv_t)[3]
+        x, M, L, _ = _cpu_stats(logits.reshape(-1, V), inv_t)
         ctx.inv_t = inv_t
         ctx.save_for_backward(logits, ids, teacher)
         some, at, q, logq = _cpu_teacher(ids.reshape(-1, K), teacher.reshape(-1, K), V, inv_t,
-                                         lp.dtype)
-        each = torch.where(q == 0, 0.0, q * (logq - lp.gather(1, at)))
+                                         x.dtype)
+        # q (log q - lp), q taken into lp's product first: csrc/vocab.hip's distill_row
+        dead = (M == -math.inf)[:, None]
+        c = torch.where(dead, -math.inf, x.gather(1, at) - M[:, None])
+        each = q * (logq + torch.where(dead, 0.0, L[:, None])) - q * c * inv_t
+        each = torch.where(q == 0, 0.0, each)
         return torch.where(some, each.sum(1), 0.0).view(logits.shape[:-1])
 
     @staticmethod

@@ -4,7 +4,8 @@ off.  U = 2^-24 is one rounding: an exponential of d costs 4 |d| + 4 of them
 (difference, scale, the factor log2 e, the exponential itself), a sum over V
 values a chain of at most V / 256 + 24.  FLUSH: the hardware's exponential gives
 0 where the result would be subnormal, so a probability may be off by the
-smallest normal number."""
+smallest normal number (which counts where a teacher's mass of 1e-39 meets a
+log probability of -1e38)."""
 import math
 
 import torch
@@ -133,7 +134,7 @@ def distill(x, ids, teacher, T=1.0, g=None):
                 continue
             lq = (b - top) / T - math.log(Z)
             lp, e_lp = (-INF, 0.0) if r is None else (float(r[0][a]), float(r[1][a]))
-            e_q = q * (el + 4 * U * (1 + abs(lq)))
+            e_q = q * (el + 4 * U * (1 + abs(lq))) + FLUSH
             loss += q * (lq - lp)
             if math.isfinite(lp):
                 err += e_q * abs(lq - lp) + q * (el + e_lp + (K + 4) * U * (abs(lq) + abs(lp)))

@@ -198,6 +198,13 @@ def test_gradients_of_means_and_parts():
                  oracle.distill(x.detach().reshape(6, 301), ids, q, g=sixth.expand(6))['dlogits'])
 
 
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('T', [0.3, 1.0])
+def test_teacher_mass_on_masked_tokens(dtype, T):
+    from tests.test_vocab import masked_by_lowest
+    check_distill(*masked_by_lowest(dtype, DEV), T)
+
+
 def test_bad_ids_are_nan_and_stay_in_their_row():
     x = logits(5, 260, BF16).requires_grad_(True)
     t = torch.tensor([260, 3, -1, 2 ** 40, -100], device=DEV)

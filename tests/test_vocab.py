@@ -86,6 +86,23 @@ def test_teacher_rows():
     oracle.check('dlogits', torch.autograd.grad(loss, x, g)[0], o['dlogits'])
 
 
+def masked_by_lowest(dtype, device='cpu'):
+    """Rows of which the teacher's tokens are partly masked by the type's lowest
+    value, its mass on them from nearly all to nearly nothing."""
+    x = torch.randn(4, 40, generator=torch.Generator().manual_seed(0))
+    x[:, 1::3] = torch.finfo(dtype).min
+    ids = torch.tensor([[0, 1, 4], [3, 4, 7], [2, 5, 1], [0, 10, 2]])
+    q = torch.tensor([[20.0, -3, 0], [30.0, -1, -2], [1.0, 2, -24], [1.0, 0, -1]])
+    return x.to(dtype).to(device), ids.to(device), q.to(device)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16, F16])
+@pytest.mark.parametrize('T', [0.3, 1.0])
+def test_teacher_mass_on_masked_tokens(dtype, T):
+    x, ids, q = masked_by_lowest(dtype)
+    oracle.check('loss', vocab.topk_distill_loss(x, ids, q, T), oracle.distill(x, ids, q, T)['loss'])
+
+
 def test_targets_out_of_range_are_nan():
     x = torch.randn(4, 6, requires_grad=True)
     t = torch.tensor([6, -1, 3, -100])

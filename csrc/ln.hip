@@ -355,11 +355,11 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
       float g[E];
       // x and z are read for the last time: s is what the backward pass reads
       // (16384 x 4096 fp16: 104 -> 85 us)
-      load_all<DT, TAIL, true, TR == 16 && TAIL, R>(x, t0, step, D, raw);
+      load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(x, t0, step, D, raw);
       if (a.zdt == DT) {
         const AS1 raw_t* z = gptr((const raw_t*)a.z) + row * a.ldz;
         u32x4n zraw[R];
-        load_all<DT, TAIL, true, TR == 16 && TAIL, R>(z, t0, step, D, zraw);
+        load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(z, t0, step, D, zraw);
 #pragma unroll
         for (int r = 0; r < R; ++r)
           vec_to_f32<DT>(clip_vec<DT, TAIL>(zraw[r], t0 + r * step, D), g + r * V);
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
         if (live) store_vec<DT, TAIL>(gptr((raw_t*)a.s) + row * D, i, D, f + r * V);
       }
     } else {
-      load_all<DT, TAIL, false, TR == 16 && TAIL, R>(x, t0, step, D, raw);
+      load_all<DT, TAIL, false, E == 8 && TR == 16 && TAIL, R>(x, t0, step, D, raw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(raw[r], t0 + r * step, D), f + r * V);
@@ -440,12 +440,12 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
     const AS1 raw_t* ds = gptr((const raw_t*)a.ds) + row * a.ldds;
     float h[E], g[E];
     u32x4n sraw[R], eraw[R];
-    load_all<DT, TAIL, true, TR == 16 && TAIL, R>(s, t0, step, D, sraw);
-    if (a.ds) load_all<DT, TAIL, true, TR == 16 && TAIL, R>(ds, t0, step, D, eraw);
+    load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(s, t0, step, D, sraw);
+    if (a.ds) load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(ds, t0, step, D, eraw);
     if (a.ydt == DT) {
       const AS1 raw_t* dy = gptr((const raw_t*)a.dy) + row * a.lddy;
       u32x4n graw[R];
-      load_all<DT, TAIL, true, TR == 16 && TAIL, R>(dy, t0, step, D, graw);
+      load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(dy, t0, step, D, graw);
 #pragma unroll
       for (int r = 0; r < R; ++r)
         vec_to_f32<DT>(clip_vec<DT, TAIL>(graw[r], t0 + r * step, D), g + r * V);
@@ -546,25 +546,27 @@ __global__ __launch_bounds__(1024) void ln_param_sum_kernel(const Bwd a) {
 
 bool dtype_ok(int dt) { return dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16; }
 
-// Threads and elements a row (TR, E): the narrowest that hold D.
 constexpr long long LONG_ROW = 16384;     // longer rows: the kernels that loop over the row
 
-#define LN_SIZES(F) F(16, 8) F(32, 8) F(64, 8) F(64, 16) F(128, 16) F(256, 16) F(512, 16) F(1024, 16)
+// Threads and elements a row (TR, E): the first that holds D.  24 elements a thread
+// stand where a class of 16 with twice the threads would be half empty and is slower
+// (us with 16 | with 24; fp16):
+//   forward    131072 x 300 62 | 52, 16384 x 4104 79 | 69; but 32768 x 2560 72 | 75,
+//              8192 x 10240 90 | 97, and with z 32768 x 1100 75 | 84
+//   backward   32768 x 1280 84 | 73, 32768 x 2560 156 | 130, 16384 x 4104 157 | 121,
+//              8192 x 10240 159 | 142; but 131072 x 300 101 | 141
+// (The backward pass of more than 12288 elements, 16 of 1024 threads | 32 of 512: 8192 x
+// 14336 194 | 185, 4096 x 16384 fp32 274 | 217.)
+#define LN_FWD_SIZES(F) \
+  F(16, 8) F(32, 8) F(16, 24) F(64, 8) F(64, 16) F(128, 16) F(256, 16) F(256, 24) F(512, 16) F(1024, 16)
+#define LN_BWD_SIZES(F) \
+  F(16, 8) F(32, 8) F(64, 8) F(64, 16) F(64, 24) F(128, 16) F(128, 24) F(256, 16) F(256, 24) \
+  F(512, 16) F(512, 24) F(512, 32)
 
 bool looped(long long D) { return D > LONG_ROW; }
 
-// threads a row
-int row_threads(long long D) {
-  int n = 0;
-#define F(TR, E) if (!n && D <= TR * E) n = TR;
-  LN_SIZES(F)
-#undef F
-  return n;
-}
-
 // workgroups that stride over the rows: at most `cap` of 256 threads (fewer, wider ones alike)
-long long row_blocks(long long rows, long long D, long long cap) {
-  const int tr = row_threads(D);
+long long row_blocks(long long rows, int tr, long long cap) {
   const long long per = tr < 256 ? 256 / tr : 1, most = tr > 256 ? cap * 256 / tr : cap;
   const long long n = (rows + per - 1) / per;
   return n < most ? n : most;
@@ -572,20 +574,25 @@ long long row_blocks(long long rows, long long D, long long cap) {
 
 constexpr long long FWD_BLOCKS = 4096;
 // A workgroup leaves 8 D bytes of sums: fewer of them for longer rows (us with
-// 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 131072 x
-// 512 fp16 117 | 104, 1048576 x 64 fp16 186 | 142).  Rows of 1024 threads again
-// need 1024, a workgroup for every CU (8192 x 16384 fp16 342 | 224).
-long long bwd_blocks(long long D) { return D > 512 && D <= 8192 ? 512 : 1024; }
+// 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 8192 x 12000
+// fp16 167 | 175, 131072 x 512 fp16 117 | 104, 1048576 x 64 fp16 186 | 142).
+long long bwd_blocks(long long rows, long long D, int tr) {
+  return row_blocks(rows, tr, D > 512 ? 512 : 1024);
+}
 
 int param_chunks(long long rows, long long D) {
-  if (!looped(D)) return (int)row_blocks(rows, D, bwd_blocks(D));
+  if (!looped(D)) {
+#define F(TR, E) if (D <= TR * E) return (int)bwd_blocks(rows, D, TR);
+    LN_BWD_SIZES(F)
+#undef F
+  }
   const long long c = (rows + 63) / 64;
   return (int)(c < 512 ? c : 512);
 }
 
 template <int DT, int TR, int E>
 void launch_fwd(const Fwd& a, hipStream_t st) {
-  const dim3 grid((unsigned)row_blocks(a.rows, a.D, FWD_BLOCKS)), block(RowSum<TR>::BT);
+  const dim3 grid((unsigned)row_blocks(a.rows, TR, FWD_BLOCKS)), block(RowSum<TR>::BT);
   if (a.D % row_vec<DT>())
     hipLaunchKernelGGL((ln_fwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
   else
@@ -593,7 +600,7 @@ void launch_fwd(const Fwd& a, hipStream_t st) {
 }
 template <int DT, int TR, int E>
 void launch_bwd(const Bwd& a, hipStream_t st) {
-  const dim3 grid((unsigned)row_blocks(a.rows, a.D, bwd_blocks(a.D))), block(RowSum<TR>::BT);
+  const dim3 grid((unsigned)bwd_blocks(a.rows, a.D, TR)), block(RowSum<TR>::BT);
   if (a.D % row_vec<DT>())
     hipLaunchKernelGGL((ln_bwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
   else
@@ -604,10 +611,8 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
     hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
     return;
   }
-  const int n = row_threads(a.D);
-  bool done = false;
-#define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_fwd<DT, TR, E>(a, st); done = true; }
-  LN_SIZES(F)
+#define F(TR, E) if (a.D <= TR * E) return launch_fwd<DT, TR, E>(a, st);
+  LN_FWD_SIZES(F)
 #undef F
 }
 template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
@@ -620,10 +625,8 @@ template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
                          dim3((unsigned)((a.D + cols - 1) / cols), a.chunks), dim3(NT), 0, st, a);
     return;
   }
-  const int n = row_threads(a.D);
-  bool done = false;
-#define F(TR, E) if (!done && n == TR && a.D <= TR * E) { launch_bwd<DT, TR, E>(a, st); done = true; }
-  LN_SIZES(F)
+#define F(TR, E) if (a.D <= TR * E) return launch_bwd<DT, TR, E>(a, st);
+  LN_BWD_SIZES(F)
 #undef F
 }
 

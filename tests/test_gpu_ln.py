@@ -117,6 +117,18 @@ def test_forward_and_gradients(shape, xt, zt):
     run_case(shape, xt, zt)
 
 
+# around the ends of the size classes, more rows than one pass of the workgroups
+EDGES = [(2100, 257), (70, 384), (70, 385), (70, 1025), (2100, 1536), (70, 1537), (600, 2500),
+         (70, 4096), (1031, 4097), (70, 6144), (70, 6145), (300, 8193), (40, 12288), (530, 12290),
+         (9, 16383)]
+
+
+@pytest.mark.parametrize('shape', EDGES)
+@pytest.mark.parametrize('xt,zt', [(F32, F32), (BF16, BF16), (F16, None), (BF16, F32)])
+def test_ends_of_the_size_classes(shape, xt, zt):
+    run_case(shape, xt, zt)
+
+
 @pytest.mark.parametrize('shape', [(3, 2), (70, 650), (2, 16387)])
 @pytest.mark.parametrize('xt,zt', MIXED)
 def test_mixed_streams(shape, xt, zt):

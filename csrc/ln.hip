@@ -329,8 +329,8 @@ __device__ __forceinline__ void store_other(void* p, long long off, int dt, int 
 
 // Bound by HBM: x and z in, s and y out.  32768 x 8192 bf16 385 us (5.6 TB/s), 8192
 // x 4096 fp32 82 us (6.5 TB/s), without z 43 us (6.2 TB/s); a row that fills its
-// registers by half or starts at an odd element is slower (16384 x 4104 fp16 76 us,
-// x 4097 88 us, x 4096 49 us).  One row of 512: 2 us; 700 x 650 fp32: 5.8 us.
+// registers by two thirds or starts at an odd element is slower (16384 x 4104 fp16 61
+// us, x 4097 81 us, x 4096 48 us).  One row of 512: 2 us; 700 x 650 fp32: 5.8 us.
 template <int DT, int TR, int E, bool TAIL>
 __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
@@ -417,8 +417,8 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
 // dx (and dz), and the workgroup's rows' part of dw and db in registers: two
 // floats an element, added over the workgroup's row groups at the end.  Bound by
 // HBM: dy, ds and s in, dx out.  32768 x 8192 bf16 380 us (5.7 TB/s), 65536 x 650
-// fp32 134 us (5.1 TB/s), 700 x 650 fp32 6.7 us.  Rows of more than 8192 elements
-// spill some registers (1024 threads of 128): 8192 x 16384 fp16 224 us (4.8 TB/s).
+// fp32 134 us (5.1 TB/s), 700 x 650 fp32 6.7 us.  16384 x 4104 fp16 121 us
+// (4.5 TB/s), 8192 x 16384 fp16 220 us (4.9 TB/s; in fp32 some registers spill: 5.0).
 template <int DT, int TR, int E, bool TAIL>
 __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
@@ -551,17 +551,25 @@ constexpr long long LONG_ROW = 16384;     // longer rows: the kernels that loop 
 // Threads and elements a row (TR, E): the first that holds D.  24 elements a thread
 // stand where a class of 16 with twice the threads would be half empty and is slower
 // (us with 16 | with 24; fp16):
-//   forward    131072 x 300 62 | 52, 16384 x 4104 79 | 69; but 32768 x 2560 72 | 75,
-//              8192 x 10240 90 | 97, and with z 32768 x 1100 75 | 84
-//   backward   32768 x 1280 84 | 73, 32768 x 2560 156 | 130, 16384 x 4104 157 | 121,
-//              8192 x 10240 159 | 142; but 131072 x 300 101 | 141
+//   forward    131072 x 300 52 | 47, 65536 x 650 49 | 41, 32768 x 1280 42 | 34,
+//              32768 x 2560 73 | 69, 16384 x 4104 79 | 61; but 8192 x 10240 85 | 103
+//   backward   65536 x 650 96 | 83, 32768 x 1280 84 | 73, 32768 x 2560 156 | 130, 16384 x
+//              4104 157 | 121, 8192 x 10240 159 | 142; but 131072 x 300 101 | 141
+// In fp32 they gain nothing (16384 x 5120 forward 124 | 131, backward 125 | 124) and cost
+// time where there are few rows (700 x 650: 5.8 | 7.5 and 6.7 | 9.2), so there they are
+// taken only for wide rows' gradients.
 // (The backward pass of more than 12288 elements, 16 of 1024 threads | 32 of 512: 8192 x
 // 14336 194 | 185, 4096 x 16384 fp32 274 | 217.)
 #define LN_FWD_SIZES(F) \
-  F(16, 8) F(32, 8) F(16, 24) F(64, 8) F(64, 16) F(128, 16) F(256, 16) F(256, 24) F(512, 16) F(1024, 16)
+  F(16, 8) F(32, 8) F(16, 24) F(64, 8) F(32, 24) F(64, 16) F(64, 24) F(128, 16) F(128, 24) \
+  F(256, 16) F(256, 24) F(512, 16) F(1024, 16)
 #define LN_BWD_SIZES(F) \
-  F(16, 8) F(32, 8) F(64, 8) F(64, 16) F(64, 24) F(128, 16) F(128, 24) F(256, 16) F(256, 24) \
+  F(16, 8) F(32, 8) F(64, 8) F(32, 24) F(64, 16) F(64, 24) F(128, 16) F(128, 24) F(256, 16) F(256, 24) \
   F(512, 16) F(512, 24) F(512, 32)
+
+constexpr bool size_of_type(int dt, int tr, int e) {
+  return dt != KDT_F32 || e != 24 || tr == 512;
+}
 
 bool looped(long long D) { return D > LONG_ROW; }
 
@@ -572,7 +580,13 @@ long long row_blocks(long long rows, int tr, long long cap) {
   return n < most ? n : most;
 }
 
-constexpr long long FWD_BLOCKS = 4096;
+// A workgroup loads the weights once for all its rows.  With 24 elements of 16 bits a
+// thread no more workgroups than run at once, three a CU (us with 4096 | 768: 5001 x
+// 4097 fp16 33 | 25, 16384 x 4104 71 | 60, 32768 x 1280 38 | 34); of 512 threads and
+// more half as many (8192 x 8191 76 | 64).
+long long fwd_blocks(long long rows, int tr, int e) {
+  return row_blocks(rows, tr, e == 24 ? 768 : tr >= 512 ? 2048 : 4096);
+}
 // A workgroup leaves 8 D bytes of sums: fewer of them for longer rows (us with
 // 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 8192 x 12000
 // fp16 167 | 175, 131072 x 512 fp16 117 | 104, 1048576 x 64 fp16 186 | 142).
@@ -580,9 +594,9 @@ long long bwd_blocks(long long rows, long long D, int tr) {
   return row_blocks(rows, tr, D > 512 ? 512 : 1024);
 }
 
-int param_chunks(long long rows, long long D) {
+int param_chunks(long long rows, long long D, int dt) {
   if (!looped(D)) {
-#define F(TR, E) if (D <= TR * E) return (int)bwd_blocks(rows, D, TR);
+#define F(TR, E) if (D <= TR * E && size_of_type(dt, TR, E)) return (int)bwd_blocks(rows, D, TR);
     LN_BWD_SIZES(F)
 #undef F
   }
@@ -592,7 +606,7 @@ int param_chunks(long long rows, long long D) {
 
 template <int DT, int TR, int E>
 void launch_fwd(const Fwd& a, hipStream_t st) {
-  const dim3 grid((unsigned)row_blocks(a.rows, TR, FWD_BLOCKS)), block(RowSum<TR>::BT);
+  const dim3 grid((unsigned)fwd_blocks(a.rows, TR, E)), block(RowSum<TR>::BT);
   if (a.D % row_vec<DT>())
     hipLaunchKernelGGL((ln_fwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
   else
@@ -611,7 +625,8 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
     hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
     return;
   }
-#define F(TR, E) if (a.D <= TR * E) return launch_fwd<DT, TR, E>(a, st);
+#define F(TR, E) \
+  if constexpr (size_of_type(DT, TR, E)) if (a.D <= TR * E) return launch_fwd<DT, TR, E>(a, st);
   LN_FWD_SIZES(F)
 #undef F
 }
@@ -625,7 +640,8 @@ template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
                          dim3((unsigned)((a.D + cols - 1) / cols), a.chunks), dim3(NT), 0, st, a);
     return;
   }
-#define F(TR, E) if (a.D <= TR * E) return launch_bwd<DT, TR, E>(a, st);
+#define F(TR, E) \
+  if constexpr (size_of_type(DT, TR, E)) if (a.D <= TR * E) return launch_bwd<DT, TR, E>(a, st);
   LN_BWD_SIZES(F)
 #undef F
 }
@@ -633,8 +649,8 @@ template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
 }  // namespace
 
 // floats of the workspace of one backward call that asks for dw or db
-KFAC_API long long kfac_ln_ws_floats(long long rows, long long D) {
-  return 2LL * param_chunks(rows, D) * D;
+KFAC_API long long kfac_ln_ws_floats(long long rows, long long D, int sdt) {
+  return 2LL * param_chunks(rows, D, sdt) * D;
 }
 
 KFAC_API int kfac_ln_forward(const KfacLnFwd* args, hipStream_t stream) {
@@ -657,7 +673,7 @@ KFAC_API int kfac_ln_backward(const KfacLnBwd* args, hipStream_t stream) {
       ((a.dw || a.db) && !a.part))
     return -2;
   if (!a.dw && !a.db) a.part = nullptr;
-  a.chunks = param_chunks(a.rows, a.D);
+  a.chunks = param_chunks(a.rows, a.D, a.sdt);
   if (a.sdt == KDT_F32) launch_bwd_any<KDT_F32>(a, stream);
   else if (a.sdt == KDT_BF16) launch_bwd_any<KDT_BF16>(a, stream);
   else launch_bwd_any<KDT_F16>(a, stream);

@@ -67,7 +67,7 @@ struct KfacVocabBwd {
 extern "C" {
 int kfac_ln_forward(const KfacLnFwd* args, ihipStream_t* stream);
 int kfac_ln_backward(const KfacLnBwd* args, ihipStream_t* stream);
-long long kfac_ln_ws_floats(long long rows, long long D);
+long long kfac_ln_ws_floats(long long rows, long long D, int sdt);
 int kfac_vocab_forward(const KfacVocabFwd* args, ihipStream_t* stream);
 int kfac_vocab_backward(const KfacVocabBwd* args, ihipStream_t* stream);
 long long kfac_vocab_ws_bytes(int dt, long long rows, long long V, int k);

@@ -127,7 +127,7 @@ NormGrad norm_backward(const Tensor& dy, const Tensor& ds, const Tensor& s, Tens
   if (need_w) r.dw = contiguous_like(weight, weight.scalar_type());
   if (need_b) r.db = contiguous_like(bias, bias.scalar_type());
   if (need_w || need_b)
-    part = at::empty({(int64_t)kfac_ln_ws_floats(rows, D)}, s.options().dtype(at::kFloat));
+    part = at::empty({(int64_t)kfac_ln_ws_floats(rows, D, code(s.scalar_type()))}, s.options().dtype(at::kFloat));
   const Rows gr(dy, rows, D), er(ds, rows, D), sr(s, rows, D);
   if (weight.defined()) weight = weight.contiguous();
   KfacLnBwd a = {};

@@ -583,9 +583,11 @@ long long row_blocks(long long rows, int tr, long long cap) {
 // A workgroup loads the weights once for all its rows.  With 24 elements of 16 bits a
 // thread no more workgroups than run at once, three a CU (us with 4096 | 768: 5001 x
 // 4097 fp16 33 | 25, 16384 x 4104 71 | 60, 32768 x 1280 38 | 34); of 512 threads and
-// more half as many (8192 x 8191 76 | 64).
-long long fwd_blocks(long long rows, int tr, int e) {
-  return row_blocks(rows, tr, e == 24 ? 768 : tr >= 512 ? 2048 : 4096);
+// more half as many (8192 x 8191 76 | 64, with z 2048 x 8191 45 | 38), but where z and
+// s move as well and rows are many (32768 x 8192 bf16 397 | 409).
+long long fwd_blocks(const Fwd& a, int tr, int e) {
+  const bool half = tr >= 512 && (!a.z || a.rows < 16384);
+  return row_blocks(a.rows, tr, e == 24 ? 768 : half ? 2048 : 4096);
 }
 // A workgroup leaves 8 D bytes of sums: fewer of them for longer rows (us with
 // 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 8192 x 12000
@@ -606,7 +608,7 @@ int param_chunks(long long rows, long long D, int dt) {
 
 template <int DT, int TR, int E>
 void launch_fwd(const Fwd& a, hipStream_t st) {
-  const dim3 grid((unsigned)fwd_blocks(a.rows, TR, E)), block(RowSum<TR>::BT);
+  const dim3 grid((unsigned)fwd_blocks(a, TR, E)), block(RowSum<TR>::BT);
   if (a.D % row_vec<DT>())
     hipLaunchKernelGGL((ln_fwd_kernel<DT, TR, E, true>), grid, block, 0, st, a);
   else

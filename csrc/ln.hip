@@ -327,7 +327,7 @@ __device__ __forceinline__ void store_other(void* p, long long off, int dt, int 
   else store_as<KDT_F16, V, R>(p, off, t0, step, n, f);
 }
 
-// Bound by HBM: x and z in, s and y out.  32768 x 8192 bf16 385 us (5.6 TB/s), 8192
+// Bound by HBM: x and z in, s and y out.  32768 x 8192 bf16 397 us (5.4 TB/s), 8192
 // x 4096 fp32 82 us (6.5 TB/s), without z 43 us (6.2 TB/s); a row that fills its
 // registers by two thirds or starts at an odd element is slower (16384 x 4104 fp16 61
 // us, x 4097 81 us, x 4096 48 us).  One row of 512: 2 us; 700 x 650 fp32: 5.8 us.
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
 
 // dx (and dz), and the workgroup's rows' part of dw and db in registers: two
 // floats an element, added over the workgroup's row groups at the end.  Bound by
-// HBM: dy, ds and s in, dx out.  32768 x 8192 bf16 380 us (5.7 TB/s), 65536 x 650
+// HBM: dy, ds and s in, dx out.  32768 x 8192 bf16 385 us (5.6 TB/s), 65536 x 650
 // fp32 134 us (5.1 TB/s), 700 x 650 fp32 6.7 us.  16384 x 4104 fp16 121 us
 // (4.5 TB/s), 8192 x 16384 fp16 220 us (4.9 TB/s; in fp32 some registers spill: 5.0).
 template <int DT, int TR, int E, bool TAIL>

@@ -28,9 +28,10 @@
 //
 // Defined edges: a row whose target is `ignore` is neither read nor gives a
 // gradient (0, ids -1); a row of only -inf has logprob -inf, entropy 0 and no
-// gradient; NaN or +inf in a row, or a target out of range, makes its results
-// NaN; a teacher row without a used slot (id -1) or with only -inf gives
-// loss 0 and no gradient.
+// gradient; NaN or +inf in a row makes its results and its gradient NaN (a row of
+// only NaN, or of NaN and -inf, too), a target out of range its logprob and the
+// logprob's gradient; a teacher row without a used slot (id -1) or with only -inf
+// gives loss 0 and no gradient.
 #include "records.h"
 #include "rows.h"
 
@@ -259,7 +260,9 @@ __device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* 
   if (first) fold_any<V, ENT>(before, c1, m, s, a);
 }
 
-// (m, s, a) joined over the workgroup
+// (m, s, a) joined over the workgroup.  Maxima pass over NaN, so that a row of only
+// NaN and -inf has the maximum of a masked one: its sum is NaN, and makes the row's
+// M, and by it all that follows, NaN.
 template <int NT, bool ENT>
 __device__ __forceinline__ void join(float c1, float* red, float& m, float& s, float& a) {
   const float M = Group<NT>::max(m, red);
@@ -267,7 +270,7 @@ __device__ __forceinline__ void join(float c1, float* red, float& m, float& s, f
   const float scale = __builtin_amdgcn_exp2f(back);
   if (ENT) a = Group<NT>::sum(scale * fmaf(back, s, a), red);
   s = Group<NT>::sum(s * scale, red);
-  m = M;
+  m = s == s ? M : NAN;
 }
 
 // How many of count keys are larger than v, eight reads of LDS in flight (one by one,

@@ -15,7 +15,8 @@ bitwise reproducible, no host synchronisation; the autograd nodes are C++,
 csrc/torch_ops.cpp), CPU tensors on the same formulas in torch.  Neither op has a second derivative.
 
 What a kernel meets on the device cannot raise without a synchronisation: a
-target or id out of range makes its row's results and gradient NaN.
+target out of range makes its row's log probability and that one's gradient NaN,
+a teacher's id out of range its row's loss and gradient.
 """
 import math
 from typing import NamedTuple, Optional
@@ -168,7 +169,8 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=False, temperature=1.0
     logits); the alternatives do not.
 
     A row of only -inf (everything masked) has log probabilities -inf, entropy
-    0 and no gradient.  NaN or +inf in a row makes its results NaN.
+    0 and no gradient.  NaN or +inf in a row, also beside nothing but -inf or
+    NaN, makes its results and its gradient NaN.
     """
     inv_t = _check('token_logprobs', logits, temperature)
     if targets is not None:

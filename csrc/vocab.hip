@@ -310,6 +310,7 @@ template <int NT> struct TopShared {
   };
   int hist[256];
   int n, entries, bound;
+  int kept_n;                    // of `kept`: apart from n, which waves may still be reading
 };
 
 // The largest bound that at least k of a wave's N keys a lane reach, bit by bit
@@ -377,7 +378,7 @@ __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>:
     before(most);
   }
   sh.key[tid] = key;
-  if (tid == 0) sh.n = sh.entries = 0;
+  if (tid == 0) sh.n = sh.entries = sh.kept_n = 0;
   __syncthreads();
   if (tid < 64) {
     uint32_t own[NT / 64];
@@ -504,17 +505,14 @@ __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>:
       for (int j = 0; j < TopShared<NT>::CAND / 64; ++j)
         own[j] = tid + 64 * j < count ? (uint32_t)(sh.cand[tid + 64 * j] >> 32) : 0u;
       const uint32_t kth = kth_of_wave<TopShared<NT>::CAND / 64, LOW>(own, k);
-      if (tid == 0) {
-        sh.bound = (int)kth;
-        sh.n = 0;
-      }
+      if (tid == 0) sh.bound = (int)kth;
     }
     __syncthreads();
     const uint32_t kth = (uint32_t)sh.bound;
     for (int c = tid; c < count; c += NT)
-      if ((uint32_t)(sh.cand[c] >> 32) >= kth) sh.kept[atomicAdd(&sh.n, 1)] = sh.cand[c];
+      if ((uint32_t)(sh.cand[c] >> 32) >= kth) sh.kept[atomicAdd(&sh.kept_n, 1)] = sh.cand[c];
     __syncthreads();
-    count = sh.n;
+    count = sh.kept_n;
     cand = sh.kept;
     pad_list(sh.kept, count);
   } else {

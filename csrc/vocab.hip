@@ -43,6 +43,8 @@ typedef KfacVocabBwd Bwd;
 constexpr int TOP_MAX = 128;      // alternatives, and slots of a teacher's row
 constexpr int MAX_V = 1 << 30;    // elements of a row: 32-bit offsets within it
 constexpr int MAX_SPLITS = 64;    // workgroups a row
+// workgroups a launch, which has fewer than 2^32 threads: more rows take several launches
+constexpr long long MAX_GROUPS = 1 << 22;
 // Logits that the 256 MB of last-level cache cannot hold beside their gradient
 // are read past it (non-temporal): the backward pass would not find them there.
 // us forward + backward, streamed | not: 4096 x 131072 bf16 197 + 373 | 232 +
@@ -903,19 +905,66 @@ int fwd_splits(int dt, long long rows, long long V, int k) {
 
 bool dtype_ok(int dt) { return dt == KDT_F32 || dt == KDT_BF16 || dt == KDT_F16; }
 
+template <class T> T* at(T* p, long long n) { return p ? p + n : p; }
+const void* at(const void* p, long long n, int dt) {
+  return at((const char*)p, n * (dt == KDT_F32 ? 4 : 2));
+}
+
+// rows r0 .. r0 + rows - 1 of a
+Fwd some_rows(Fwd a, long long r0, long long rows) {
+  a.x = at(a.x, r0 * a.ld, a.dt);
+  a.targets = at(a.targets, r0);
+  a.logprob = at(a.logprob, r0);
+  a.entropy = at(a.entropy, r0);
+  a.top_lp = at(a.top_lp, r0 * a.k);
+  a.top_ids = at(a.top_ids, r0 * a.k);
+  a.stats = at(a.stats, 2 * r0);
+  a.ids = at(a.ids, r0 * a.K);
+  a.teacher = at(a.teacher, r0 * a.K, a.tdt);
+  a.loss = at(a.loss, r0);
+  a.keep_ids = at(a.keep_ids, r0 * a.K);
+  a.keep_q = at(a.keep_q, r0 * a.K);
+  a.rows = rows;
+  return a;
+}
+Bwd some_rows(Bwd a, long long r0, long long rows) {
+  a.x = at(a.x, r0 * a.ld, a.dt);
+  a.stats = at(a.stats, 2 * r0);
+  a.entropy = at(a.entropy, r0);
+  a.targets = at(a.targets, r0);
+  a.g = at(a.g, r0 * a.gs);
+  a.gh = at(a.gh, r0 * a.ghs);
+  a.keep_ids = at(a.keep_ids, r0 * a.K);
+  a.keep_q = at(a.keep_q, r0 * a.K);
+  a.dx = (void*)at(a.dx, r0 * a.V, a.dt);
+  a.rows = rows;
+  return a;
+}
+
+// one launch for each range of rows that has at most MAX_GROUPS workgroups
+template <class Args, class Launch> void each_range(const Args& a, int splits, Launch launch) {
+  const long long most = MAX_GROUPS / splits;
+  for (long long r0 = 0; r0 < a.rows; r0 += most)
+    launch(some_rows(a, r0, a.rows - r0 < most ? a.rows - r0 : most));
+}
+
 template <int DT, int MODE, bool ENT, bool TOP>
 void launch_fwd(const Fwd& a, hipStream_t st) {
   const int splits = fwd_splits(a.dt, a.rows, a.V, a.k);
   if (splits == 1 && fwd_threads(a.dt, a.rows, a.V, a.k) == 64) {
-    hipLaunchKernelGGL((vocab_fwd_kernel<DT, 64, MODE, ENT, TOP>), dim3((unsigned)a.rows),
-                       dim3(64), 0, st, a, 1, (int)a.V);
+    each_range(a, 1, [&](const Fwd& r) {
+      hipLaunchKernelGGL((vocab_fwd_kernel<DT, 64, MODE, ENT, TOP>), dim3((unsigned)r.rows),
+                         dim3(64), 0, st, r, 1, (int)r.V);
+    });
     return;
   }
   const int vec = row_vec<DT>();
   const int chunk = (int)((a.V + splits - 1) / splits + vec - 1) / vec * vec;
-  hipLaunchKernelGGL((vocab_fwd_kernel<DT, 256, MODE, ENT, TOP>),
-                     dim3((unsigned)(a.rows * splits)), dim3(256), 0, st, a, splits, chunk);
-  if (splits > 1)
+  each_range(a, splits, [&](const Fwd& r) {
+    hipLaunchKernelGGL((vocab_fwd_kernel<DT, 256, MODE, ENT, TOP>),
+                       dim3((unsigned)(r.rows * splits)), dim3(256), 0, st, r, splits, chunk);
+  });
+  if (splits > 1)                          // few rows: one range
     hipLaunchKernelGGL((vocab_join_kernel<DT, MODE, ENT, TOP>), dim3((unsigned)a.rows),
                        dim3(JOIN_NT), 0, st, a, splits);
 }
@@ -930,13 +979,15 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
 
 template <int DT> void launch_bwd(const Bwd& a, hipStream_t st) {
   const int splits = (int)((a.V + bwd_chunk<DT>() - 1) / bwd_chunk<DT>());
-  const dim3 grid((unsigned)(a.rows * splits)), block(BWD_NT);
-  if (a.keep_ids)
-    hipLaunchKernelGGL((vocab_bwd_kernel<DT, DISTILL, false>), grid, block, 0, st, a, splits);
-  else if (a.gh)
-    hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, true>), grid, block, 0, st, a, splits);
-  else
-    hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, false>), grid, block, 0, st, a, splits);
+  each_range(a, splits, [&](const Bwd& r) {
+    const dim3 grid((unsigned)(r.rows * splits)), block(BWD_NT);
+    if (r.keep_ids)
+      hipLaunchKernelGGL((vocab_bwd_kernel<DT, DISTILL, false>), grid, block, 0, st, r, splits);
+    else if (r.gh)
+      hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, true>), grid, block, 0, st, r, splits);
+    else
+      hipLaunchKernelGGL((vocab_bwd_kernel<DT, LOGPROB, false>), grid, block, 0, st, r, splits);
+  });
 }
 
 }  // namespace

@@ -21,6 +21,9 @@ typedef KfacLnFwd Fwd;
 typedef KfacLnBwd Bwd;
 
 constexpr int NT = 256, LT = 1024;     // threads: columns' sums, long rows
+// A launch has fewer than 2^32 threads: workgroups of 1024 stride over what is more
+// than this many of them.
+constexpr long long MAX_GROUPS = 1 << 16;
 
 __device__ __forceinline__ float ld_any(const void* p, long long i, int dt) {
   if (dt == KDT_F32) return ((const float*)p)[i];
@@ -93,50 +96,52 @@ __global__ __launch_bounds__(LT) void ln_fwd_long_kernel(const Fwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
   constexpr int V = row_vec<DT>(), STEP = LT * V;
   __shared__ float red[LT / 64];
-  const long long row = blockIdx.x, D = a.D, t0 = threadIdx.x * V;
-  const long long yo = row * D;
-  const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
-  float acc = 0.f;
-  for (long long i = t0; i < D; i += STEP) {
-    float f[V];
-    walk_load<DT>(x, i, D, f);
-    if (a.z) {
-      float g[V];
-      walk_other<DT>(a.z, row * a.ldz, a.zdt, i, D, g);
+  const long long D = a.D, t0 = threadIdx.x * V;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const long long yo = row * D;
+    const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
+    float acc = 0.f;
+    for (long long i = t0; i < D; i += STEP) {
+      float f[V];
+      walk_load<DT>(x, i, D, f);
+      if (a.z) {
+        float g[V];
+        walk_other<DT>(a.z, row * a.ldz, a.zdt, i, D, g);
 #pragma unroll
-      for (int e = 0; e < V; ++e)      // the sum as it is stored is what is normed
-        f[e] = DTypeTraits<DT>::to_f32(DTypeTraits<DT>::from_f32(f[e] + g[e]));
-      walk_store<DT>(a.s, yo, DT, i, D, f);
+        for (int e = 0; e < V; ++e)      // the sum as it is stored is what is normed
+          f[e] = DTypeTraits<DT>::to_f32(DTypeTraits<DT>::from_f32(f[e] + g[e]));
+        walk_store<DT>(a.s, yo, DT, i, D, f);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc += f[e];
     }
+    const AS1 raw_t* s = a.z ? gptr((const raw_t*)a.s) + yo : x;     // each thread's own stores
+    const float mu = block_sum(acc, red) / (float)D;
+    acc = 0.f;
+    for (long long i = t0; i < D; i += STEP) {
+      float f[V];
+      walk_load<DT>(s, i, D, f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc += f[e];
-  }
-  const AS1 raw_t* s = a.z ? gptr((const raw_t*)a.s) + yo : x;     // each thread's own stores
-  const float mu = block_sum(acc, red) / (float)D;
-  acc = 0.f;
-  for (long long i = t0; i < D; i += STEP) {
-    float f[V];
-    walk_load<DT>(s, i, D, f);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float d = f[e] - mu;
-      acc = fmaf(d, i + e < D ? d : 0.f, acc);
+      for (int e = 0; e < V; ++e) {
+        const float d = f[e] - mu;
+        acc = fmaf(d, i + e < D ? d : 0.f, acc);
+      }
     }
-  }
-  const float rstd = 1.f / sqrtf(block_sum(acc, red) / (float)D + a.eps);
-  for (long long i = t0; i < D; i += STEP) {
-    float f[V], w[V], b[V];
-    walk_load<DT>(s, i, D, f);
-    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
-    if (a.b) walk_other<DT>(a.b, 0, a.bdt, i, D, b);
+    const float rstd = 1.f / sqrtf(block_sum(acc, red) / (float)D + a.eps);
+    for (long long i = t0; i < D; i += STEP) {
+      float f[V], w[V], b[V];
+      walk_load<DT>(s, i, D, f);
+      if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+      if (a.b) walk_other<DT>(a.b, 0, a.bdt, i, D, b);
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      f[e] = fmaf((f[e] - mu) * rstd, a.w ? w[e] : 1.f, a.b ? b[e] : 0.f);
-    walk_store<DT>(a.y, yo, a.ydt, i, D, f);
-  }
-  if (threadIdx.x == 0 && a.mean) {
-    a.mean[row] = mu;
-    a.rstd[row] = rstd;
+      for (int e = 0; e < V; ++e)
+        f[e] = fmaf((f[e] - mu) * rstd, a.w ? w[e] : 1.f, a.b ? b[e] : 0.f);
+      walk_store<DT>(a.y, yo, a.ydt, i, D, f);
+    }
+    if (threadIdx.x == 0 && a.mean) {
+      a.mean[row] = mu;
+      a.rstd[row] = rstd;
+    }
   }
 }
 
@@ -145,37 +150,39 @@ __global__ __launch_bounds__(LT) void ln_bwd_long_kernel(const Bwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
   constexpr int V = row_vec<DT>(), STEP = LT * V;
   __shared__ float red[LT / 64];
-  const long long row = blockIdx.x, D = a.D, t0 = threadIdx.x * V;
-  const AS1 raw_t* s = gptr((const raw_t*)a.s) + row * a.lds;
-  const float mu = a.mean[row], rstd = a.rstd[row];
-  float c1 = 0.f, c2 = 0.f;
-  for (long long i = t0; i < D; i += STEP) {
-    float g[V], h[V], w[V];
-    walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
-    walk_load<DT>(s, i, D, h);
-    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+  const long long D = a.D, t0 = threadIdx.x * V;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const AS1 raw_t* s = gptr((const raw_t*)a.s) + row * a.lds;
+    const float mu = a.mean[row], rstd = a.rstd[row];
+    float c1 = 0.f, c2 = 0.f;
+    for (long long i = t0; i < D; i += STEP) {
+      float g[V], h[V], w[V];
+      walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
+      walk_load<DT>(s, i, D, h);
+      if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float v = a.w ? g[e] * w[e] : g[e];
-      c1 += v;
-      c2 = fmaf(v, (h[e] - mu) * rstd, c2);
+      for (int e = 0; e < V; ++e) {
+        const float v = a.w ? g[e] * w[e] : g[e];
+        c1 += v;
+        c2 = fmaf(v, (h[e] - mu) * rstd, c2);
+      }
     }
-  }
-  c1 = block_sum(c1, red) / (float)D;
-  c2 = block_sum(c2, red) / (float)D;
-  for (long long i = t0; i < D; i += STEP) {
-    float g[V], h[V], w[V], d[V];
-    walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
-    walk_load<DT>(s, i, D, h);
-    if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
-    if (a.ds) walk_load<DT>(gptr((const raw_t*)a.ds) + row * a.ldds, i, D, d);
+    c1 = block_sum(c1, red) / (float)D;
+    c2 = block_sum(c2, red) / (float)D;
+    for (long long i = t0; i < D; i += STEP) {
+      float g[V], h[V], w[V], d[V];
+      walk_other<DT>(a.dy, row * a.lddy, a.ydt, i, D, g);
+      walk_load<DT>(s, i, D, h);
+      if (a.w) walk_other<DT>(a.w, 0, a.wdt, i, D, w);
+      if (a.ds) walk_load<DT>(gptr((const raw_t*)a.ds) + row * a.ldds, i, D, d);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float v = a.w ? g[e] * w[e] : g[e];
-      g[e] = rstd * (v - c1 - (h[e] - mu) * rstd * c2) + (a.ds ? d[e] : 0.f);
+      for (int e = 0; e < V; ++e) {
+        const float v = a.w ? g[e] * w[e] : g[e];
+        g[e] = rstd * (v - c1 - (h[e] - mu) * rstd * c2) + (a.ds ? d[e] : 0.f);
+      }
+      walk_store<DT>(a.dx, row * D, DT, i, D, g);
+      if (a.dz) walk_store<DT>(a.dz, row * D, a.zdt, i, D, g);
     }
-    walk_store<DT>(a.dx, row * D, DT, i, D, g);
-    if (a.dz) walk_store<DT>(a.dz, row * D, a.zdt, i, D, g);
   }
 }
 
@@ -524,23 +531,26 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
 __global__ __launch_bounds__(1024) void ln_param_sum_kernel(const Bwd a) {
   __shared__ float sh[2][32][33];
   const int cx = threadIdx.x & 31, k0 = threadIdx.x >> 5;
-  const long long c = (long long)blockIdx.x * 32 + cx;
-  float dw = 0.f, db = 0.f;
-  if (c < a.D) {
+  for (long long c0 = blockIdx.x * 32LL; c0 < a.D; c0 += gridDim.x * 32LL) {
+    const long long c = c0 + cx;
+    float dw = 0.f, db = 0.f;
+    if (c < a.D) {
 #pragma unroll 4
-    for (int k = k0; k < a.chunks; k += 32) {
-      dw += a.part[2LL * k * a.D + c];
-      db += a.part[(2LL * k + 1) * a.D + c];
+      for (int k = k0; k < a.chunks; k += 32) {
+        dw += a.part[2LL * k * a.D + c];
+        db += a.part[(2LL * k + 1) * a.D + c];
+      }
     }
-  }
-  sh[0][k0][cx] = dw;
-  sh[1][k0][cx] = db;
-  __syncthreads();
-  if (k0 < 2 && c < a.D) {
-    float v = 0.f;
-    for (int k = 0; k < 32; ++k) v += sh[k0][k][cx];
-    if (k0 == 0 && a.dw) st_any(a.dw, c, a.wdt, v);
-    if (k0 == 1 && a.db) st_any(a.db, c, a.bdt, v);
+    sh[0][k0][cx] = dw;
+    sh[1][k0][cx] = db;
+    __syncthreads();
+    if (k0 < 2 && c < a.D) {
+      float v = 0.f;
+      for (int k = 0; k < 32; ++k) v += sh[k0][k][cx];
+      if (k0 == 0 && a.dw) st_any(a.dw, c, a.wdt, v);
+      if (k0 == 1 && a.db) st_any(a.db, c, a.bdt, v);
+    }
+    __syncthreads();                       // sh is written again
   }
 }
 
@@ -572,6 +582,8 @@ constexpr bool size_of_type(int dt, int tr, int e) {
 }
 
 bool looped(long long D) { return D > LONG_ROW; }
+
+unsigned groups(long long n) { return (unsigned)(n < MAX_GROUPS ? n : MAX_GROUPS); }
 
 // workgroups that stride over the rows: at most `cap` of 256 threads (fewer, wider ones alike)
 long long row_blocks(long long rows, int tr, long long cap) {
@@ -624,7 +636,7 @@ void launch_bwd(const Bwd& a, hipStream_t st) {
 }
 template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
   if (looped(a.D)) {
-    hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
+    hipLaunchKernelGGL(ln_fwd_long_kernel<DT>, dim3(groups(a.rows)), dim3(LT), 0, st, a);
     return;
   }
 #define F(TR, E) \
@@ -635,7 +647,7 @@ template <int DT> void launch_fwd_any(const Fwd& a, hipStream_t st) {
 template <int DT> void launch_bwd_any(const Bwd& a, hipStream_t st) {
   if (looped(a.D)) {
     if (a.dx)
-      hipLaunchKernelGGL(ln_bwd_long_kernel<DT>, dim3((unsigned)a.rows), dim3(LT), 0, st, a);
+      hipLaunchKernelGGL(ln_bwd_long_kernel<DT>, dim3(groups(a.rows)), dim3(LT), 0, st, a);
     const long long cols = NT * row_vec<DT>();
     if (a.part)
       hipLaunchKernelGGL(ln_param_part_kernel<DT>,
@@ -680,7 +692,7 @@ KFAC_API int kfac_ln_backward(const KfacLnBwd* args, hipStream_t stream) {
   else if (a.sdt == KDT_BF16) launch_bwd_any<KDT_BF16>(a, stream);
   else launch_bwd_any<KDT_F16>(a, stream);
   if (a.part)
-    hipLaunchKernelGGL(ln_param_sum_kernel, dim3((unsigned)((a.D + 31) / 32)), dim3(1024), 0,
-                       stream, a);
+    hipLaunchKernelGGL(ln_param_sum_kernel, dim3(groups((a.D + 31) / 32)), dim3(1024), 0, stream,
+                       a);
   return (int)hipGetLastError();
 }

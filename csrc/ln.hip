@@ -164,7 +164,7 @@ __global__ __launch_bounds__(LT) void ln_bwd_long_kernel(const Bwd a) {
       for (int e = 0; e < V; ++e) {
         const float v = a.w ? g[e] * w[e] : g[e];
         c1 += v;
-        c2 = fmaf(v, (h[e] - mu) * rstd, c2);
+        c2 = fmaf(v, (h[e] - (i + e < D ? mu : 0.f)) * rstd, c2);
       }
     }
     c1 = block_sum(c1, red) / (float)D;
@@ -463,12 +463,20 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
       vec_to_f32<DT>(clip_vec<DT, TAIL>(sraw[r], t0 + r * step, D), h + r * V);
+#pragma unroll
+    for (int e = 0; e < E; ++e) h[e] = (h[e] - mu) * rstd;
+    // past the row's end g is 0 and h is (0 - mu) rstd, to be 0 too where that is no
+    // number (a select in every row: 16384 x 4097 fp16 106 -> 118 us)
+    if (__any(!(fabsf(mu * rstd) < INFINITY))) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (t0 + e / V * step + e % V >= D) h[e] = 0.f;
+    }
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      h[e] = (h[e] - mu) * rstd;
       if (!live) g[e] = 0.f;
-      dw[e] = fmaf(g[e], h[e], dw[e]);           // past the row's end g is 0
+      dw[e] = fmaf(g[e], h[e], dw[e]);
       db[e] += g[e];
       g[e] *= w[e];
       c1 += g[e];

@@ -38,10 +38,12 @@ _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def eligible(x, normalized_shape, weight=None, bias=None, z=None):
     """True where the kernels run (see the module's text)."""
-    if not (ENABLED and x.is_cuda and x.dtype in _TYPES and x.numel() > 0):
+    # asked first: a trace warns of Python values taken from shapes
+    if not (ENABLED and x.is_cuda and x.dtype in _TYPES and
+            _lib.plain_tensors(x, z, weight, bias)):
         return False
     n = len(normalized_shape)
-    if n == 0 or x.shape[-n:] != normalized_shape or \
+    if x.numel() == 0 or n == 0 or x.shape[-n:] != normalized_shape or \
             x.numel() // math.prod(normalized_shape) >= 2 ** 31:
         return False
     if z is not None and (z.shape != x.shape or z.dtype not in _TYPES or z.device != x.device):
@@ -50,7 +52,7 @@ def eligible(x, normalized_shape, weight=None, bias=None, z=None):
         if p is not None and (p.dtype not in _TYPES or p.device != x.device or
                               p.shape != normalized_shape):
             return False
-    return _lib.plain_tensors(x, z, weight, bias)
+    return True
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, z=None):

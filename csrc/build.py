@@ -7,8 +7,10 @@ files under build/, links them into
 `distributed_kfac_pytorch_amd/_native/libkfac_hip.so` (plain C ABI, loaded
 through ctypes by ops/_lib.py; no torch headers, no hipify).  csrc/torch_ops.cpp
 (host code only: autograd nodes over the C ABI) becomes
-`_native/libkfac_torch.so` with the host compiler and torch's headers.  Rebuilds
-only when a source or header is newer than the library.
+`_native/libkfac_torch.so` with the host compiler and torch's headers; it belongs
+to the torch that it was built with, whose version stands in
+`libkfac_torch.so.sources` (ops/_lib.py compares it).  Rebuilds only when a source
+or header is newer than the library, or torch is another one.
 """
 import argparse
 import concurrent.futures
@@ -83,14 +85,20 @@ def compile_optional():
 def build_torch_ops(force=False, verbose=True):
     src = os.path.join(CSRC, 'torch_ops.cpp')
     deps = [src, os.path.join(CSRC, 'records.h')]
-    if not force and not _stale(TORCH_LIB, deps):
-        return TORCH_LIB
+    stamp = TORCH_LIB + '.sources'
     try:
         import torch
         from torch.utils import cpp_extension
-    except ImportError:           # an isolated build: the operators on GPU tensors will say so
-        print('torch not found: the kernels are built, their torch operators are not')
+        hip = torch.version.hip
+    except ImportError:
+        hip = None
+    if hip is None:               # an isolated build: ops/_lib.py says so on GPU tensors
+        print('no torch for ROCm found: the kernels are built, their torch operators are not '
+              '(pip install --no-build-isolation builds them with the installed torch)')
         return None
+    same = os.path.exists(stamp) and open(stamp).read() == torch.__version__
+    if not force and same and not _stale(TORCH_LIB, deps):
+        return TORCH_LIB
     rocm = os.path.dirname(os.path.dirname(HIPCC)) if os.path.isabs(HIPCC) else '/opt/rocm'
     tmp = TORCH_LIB + '.tmp'
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared',
@@ -104,6 +112,8 @@ def build_torch_ops(force=False, verbose=True):
     if r.returncode != 0:
         raise RuntimeError('host compiler failed:\n{}\n{}'.format(' '.join(cmd), r.stderr))
     os.replace(tmp, TORCH_LIB)
+    with open(stamp, 'w') as f:
+        f.write(torch.__version__)
     if verbose:
         print('built', TORCH_LIB)
     return TORCH_LIB

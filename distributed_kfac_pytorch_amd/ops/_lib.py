@@ -10,6 +10,7 @@ used only for CPU tensors).
 import ctypes
 import os
 import threading
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -22,6 +23,7 @@ _lock = threading.Lock()
 _lib = None
 _load_error = None
 _torch_ops = None
+_torch_ops_found = None
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 
@@ -227,16 +229,43 @@ def use_native(t):
 
 def torch_ops():
     """torch.ops.kfac_hip: the operators of csrc/torch_ops.cpp (autograd nodes in
-    C++ over the same library); raises (never falls back) when it is missing."""
+    C++ over the same library); raises (never falls back) when it is missing or
+    was built with another torch."""
     global _torch_ops
     if _torch_ops is None:
         lib()
+        what = 'distributed_kfac_pytorch_amd torch operators '
+        again = '(run `python csrc/build.py`, or pip install --no-build-isolation)'
         if not os.path.exists(TORCH_LIB_PATH):
-            raise RuntimeError('distributed_kfac_pytorch_amd torch operators not built: {} '
-                               '(run `python csrc/build.py`)'.format(TORCH_LIB_PATH))
-        torch.ops.load_library(TORCH_LIB_PATH)
+            raise RuntimeError(what + 'not built: {} {}'.format(TORCH_LIB_PATH, again))
+        stamp = TORCH_LIB_PATH + '.sources'
+        if os.path.exists(stamp):
+            with open(stamp) as f:
+                built = f.read()
+            if built != torch.__version__:
+                raise RuntimeError(what + 'built with torch {}, this is {} {}'.format(
+                    built, torch.__version__, again))
+        try:
+            torch.ops.load_library(TORCH_LIB_PATH)
+        except OSError as e:
+            raise RuntimeError(what + 'not loaded: {} {}'.format(e, again))
         _torch_ops = torch.ops.kfac_hip
     return _torch_ops
+
+
+def has_torch_ops():
+    """Whether torch_ops() has what it needs; a warning, once, where it has not --
+    for what torch can do without them.  The kernel library itself is required."""
+    global _torch_ops_found
+    if _torch_ops_found is None:
+        lib()
+        try:
+            torch_ops()
+            _torch_ops_found = True
+        except RuntimeError as e:
+            warnings.warn("{}: torch's own layer norm runs instead".format(e))
+            _torch_ops_found = False
+    return _torch_ops_found
 
 
 def plain_tensors(*tensors):

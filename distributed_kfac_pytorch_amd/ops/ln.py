@@ -15,7 +15,8 @@ the autograd node is C++, csrc/torch_ops.cpp); anything else (CPU tensors, fp64,
 tensor subclasses, z of another shape, functorch transforms, dispatch modes,
 traces) takes the two torch operations.
 Unlike F.layer_norm, the weights may have another type than x.
-`KFAC_FUSED_LN=0` disables the kernels.
+`KFAC_FUSED_LN=0` disables the kernels.  An installation that was built without
+torch, or with another one, has no such node: torch's operations run, with a warning.
 
 A second derivative (create_graph=True) is taken through elementary operations.
 K-FAC hooks Conv2d / Linear only; a layer norm is not preconditioned
@@ -52,7 +53,7 @@ def eligible(x, normalized_shape, weight=None, bias=None, z=None):
         if p is not None and (p.dtype not in _TYPES or p.device != x.device or
                               p.shape != normalized_shape):
             return False
-    return True
+    return _lib.has_torch_ops()
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5, z=None):

@@ -114,6 +114,11 @@ def load_teacher(args, ntokens, device):
     return teacher.to(device).eval().requires_grad_(False)
 
 
+def score(out, targets, **kw):
+    """token_logprobs of a batch's targets, flat as get_batch gives them."""
+    return token_logprobs(out, targets.view(out.shape[:-1]), **kw)
+
+
 def distill_loss(args, out, teacher_out):
     """T^2 times the mean divergence from the teacher's likeliest tokens: T^2 keeps
     the gradient's size over temperatures."""
@@ -178,11 +183,13 @@ def main(argv=None):
             data, targets = get_batch(train, i, args.bptt)
             optimizer.zero_grad()
             out, hidden = run_model(ddp, data, hidden, args)
-            loss = criterion(out.reshape(-1, out.size(-1)), targets)
-            if teacher is not None:
+            if teacher is None:
+                loss = criterion(out.reshape(-1, out.size(-1)), targets)
+            else:
                 with torch.no_grad():
                     t_out, t_hidden = run_model(teacher, data, t_hidden, args)
-                loss = torch.lerp(loss, distill_loss(args, out, t_out), args.distill_weight)
+                loss = torch.lerp(-score(out, targets).logprobs.mean(),
+                                  distill_loss(args, out, t_out), args.distill_weight)
             loss.backward()
             torch.nn.utils.clip_grad_norm_(model.parameters(), args.clip)
             if pre is not None:
@@ -196,8 +203,8 @@ def main(argv=None):
             for i in bptt_batches(val, args.bptt):
                 data, targets = get_batch(val, i, args.bptt)
                 out, hidden = run_model(model, data, hidden, args)
-                val_m.update(criterion(out.reshape(-1, out.size(-1)), targets))
-                r = token_logprobs(out, top_k=1, entropy=True)
+                r = score(out, targets, top_k=1, entropy=True)     # one pass over the logits
+                val_m.update(-r.logprobs.mean())
                 ent_m.update(r.entropy.mean())
                 top_m.update((r.top_ids.reshape(-1) == targets).float().mean())
         sched.step()

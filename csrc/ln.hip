@@ -46,6 +46,13 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   return r;
 }
 
+// A power of two below 1 / D: elements times it have a sum within fp32 wherever they
+// are (a row masked by its type's lowest value); what else it changes is the lowest
+// bits of terms below 2^-126, far below a variance's square root in fp32.
+__device__ __forceinline__ float sum_scale(long long D) {
+  return ldexpf(1.f, __clzll(D) - 64);
+}
+
 // Rows that no workgroup's registers hold: the workgroup walks the row, once for
 // each statistic and once for the result; from the second time on it comes from a
 // cache.  1024 x 65536 fp16: 86 us forward (3.1 TB/s of what has to move), 226 us
@@ -97,6 +104,7 @@ __global__ __launch_bounds__(LT) void ln_fwd_long_kernel(const Fwd a) {
   constexpr int V = row_vec<DT>(), STEP = LT * V;
   __shared__ float red[LT / 64];
   const long long D = a.D, t0 = threadIdx.x * V;
+  const float scale = sum_scale(D);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const long long yo = row * D;
     const AS1 raw_t* x = gptr((const raw_t*)a.x) + row * a.ldx;
@@ -113,10 +121,10 @@ __global__ __launch_bounds__(LT) void ln_fwd_long_kernel(const Fwd a) {
         walk_store<DT>(a.s, yo, DT, i, D, f);
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc += f[e];
+      for (int e = 0; e < V; ++e) acc = fmaf(f[e], scale, acc);
     }
     const AS1 raw_t* s = a.z ? gptr((const raw_t*)a.s) + yo : x;     // each thread's own stores
-    const float mu = block_sum(acc, red) / (float)D;
+    const float mu = block_sum(acc, red) / ((float)D * scale);
     acc = 0.f;
     for (long long i = t0; i < D; i += STEP) {
       float f[V];
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
   __shared__ float red[2][BT / 64];
   const int t = threadIdx.x % TR, sub = threadIdx.x / TR;
   const int D = (int)a.D, t0 = t * V, step = TR * V;
-  const float inv_d = 1.f / (float)D;
+  const float inv_d = 1.f / (float)D, scale = sum_scale(D);
   float w[E], b[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) { w[e] = 1.f; b[e] = 0.f; }
@@ -391,8 +399,8 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
     }
     float acc = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc += f[e];
-    const float mu = RowSum<TR>::sum(acc, red[0]) / (float)D;    // exact for a constant row
+    for (int e = 0; e < E; ++e) acc = fmaf(f[e], scale, acc);
+    const float mu = RowSum<TR>::sum(acc, red[0]) / ((float)D * scale);    // exact for a constant row
     acc = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r)

@@ -269,16 +269,14 @@ def has_torch_ops():
 
 
 def plain_tensors(*tensors):
-    """True where raw pointers may be taken: ordinary tensors (no subclasses, not
-    nested: a nested tensor has no one shape), and no functorch transform,
-    forward-mode level, dispatch mode or trace around them (each of these needs
-    torch operations that it can see)."""
+    """True where raw pointers may be taken: ordinary tensors, and no functorch
+    transform, forward-mode level, dispatch mode or trace around them (each of
+    these needs torch operations that it can see)."""
     if torch.compiler.is_compiling() or torch._C._is_tracing() \
             or torch._C._len_torch_dispatch_stack() \
             or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
         return False
-    return all(t is None or
-               (type(t) is torch.Tensor or type(t) is torch.nn.Parameter) and not t.is_nested
+    return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter
                for t in tensors)
 
 

@@ -39,8 +39,9 @@ _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def eligible(x, normalized_shape, weight=None, bias=None, z=None):
     """True where the kernels run (see the module's text)."""
-    # asked first: a trace warns of Python values taken from shapes
-    if not (ENABLED and x.is_cuda and x.dtype in _TYPES and
+    # asked first: a trace warns of Python values taken from shapes, and a nested
+    # tensor has no shape
+    if not (ENABLED and x.is_cuda and x.dtype in _TYPES and not x.is_nested and
             _lib.plain_tensors(x, z, weight, bias)):
         return False
     n = len(normalized_shape)

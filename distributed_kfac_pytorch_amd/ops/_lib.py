@@ -276,8 +276,10 @@ def plain_tensors(*tensors):
             or torch._C._len_torch_dispatch_stack() \
             or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
         return False
-    return all(t is None or type(t) is torch.Tensor or type(t) is torch.nn.Parameter
-               for t in tensors)
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
 
 
 def stream(device=None):

@@ -12,6 +12,9 @@
 // sum are held in fp32, the variance about the mean (two passes over the row).
 // The sums over rows (dw, db) run over fixed row chunks and then over the
 // chunks in order: no atomics, bitwise reproducible.
+//
+// Times below are medians of a kernel's launches on one MI355X, three sets of inputs
+// in turn; of two sides, both with the code as it stands but for the choice.
 #include "records.h"
 #include "rows.h"
 
@@ -55,8 +58,8 @@ __device__ __forceinline__ float sum_scale(long long D) {
 
 // Rows that no workgroup's registers hold: the workgroup walks the row, once for
 // each statistic and once for the result; from the second time on it comes from a
-// cache.  1024 x 65536 fp16: 86 us forward (3.1 TB/s of what has to move), 226 us
-// backward.
+// cache.  1024 x 65536 fp16: 97 us forward (2.8 TB/s of what has to move), 226 us
+// backward, 92 of them for the weights' gradients.
 
 // V elements at i, zeros from n on
 template <int DT>
@@ -342,10 +345,11 @@ __device__ __forceinline__ void store_other(void* p, long long off, int dt, int 
   else store_as<KDT_F16, V, R>(p, off, t0, step, n, f);
 }
 
-// Bound by HBM: x and z in, s and y out.  32768 x 8192 bf16 397 us (5.4 TB/s), 8192
-// x 4096 fp32 82 us (6.5 TB/s), without z 43 us (6.2 TB/s); a row that fills its
-// registers by two thirds or starts at an odd element is slower (16384 x 4104 fp16 61
-// us, x 4097 81 us, x 4096 48 us).  One row of 512: 2 us; 700 x 650 fp32: 5.8 us.
+// Bound by HBM: x and z in, s and y out.  32768 x 8192 bf16 418 us (5.1 TB/s), 8192
+// x 4096 fp32 83 us (6.4 TB/s), without z 43 us (6.2 TB/s); a row that fills its
+// registers by two thirds or starts at an odd element is slower (16384 x 4104 fp16 74
+// us in a training step, x 4097 86 us, x 4096 66 us).  x fp32 and z bf16, as under
+// autocast: 32768 x 8192 702 us (5.4 TB/s).  One row of 512: 2 us; 700 x 650 fp32: 5.8 us.
 template <int DT, int TR, int E, bool TAIL>
 __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
@@ -369,7 +373,8 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
     if (a.z) {
       float g[E];
       // x and z are read for the last time: s is what the backward pass reads
-      // (16384 x 4096 fp16: 104 -> 85 us)
+      // (16384 x 4096 fp16 in a training step: 106 us as plain loads, 104 so; 32768 x
+      // 8192 bf16 409 and 405)
       load_all<DT, TAIL, true, E == 8 && TR == 16 && TAIL, R>(x, t0, step, D, raw);
       if (a.zdt == DT) {
         const AS1 raw_t* z = gptr((const raw_t*)a.z) + row * a.ldz;
@@ -400,7 +405,8 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
     float acc = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc = fmaf(f[e], scale, acc);
-    const float mu = RowSum<TR>::sum(acc, red[0]) / ((float)D * scale);    // exact for a constant row
+    // exact for a constant row
+    const float mu = RowSum<TR>::sum(acc, red[0]) / ((float)D * scale);
     acc = 0.f;
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -431,9 +437,10 @@ __global__ __launch_bounds__(RowSum<TR>::BT) void ln_fwd_kernel(const Fwd a) {
 
 // dx (and dz), and the workgroup's rows' part of dw and db in registers: two
 // floats an element, added over the workgroup's row groups at the end.  Bound by
-// HBM: dy, ds and s in, dx out.  32768 x 8192 bf16 385 us (5.6 TB/s), 65536 x 650
-// fp32 134 us (5.1 TB/s), 700 x 650 fp32 6.7 us.  16384 x 4104 fp16 121 us
-// (4.5 TB/s), 8192 x 16384 fp16 220 us (4.9 TB/s; in fp32 some registers spill: 5.0).
+// HBM: dy, ds and s in, dx out.  32768 x 8192 bf16 390 us (5.5 TB/s), 65536 x 650
+// fp32 127 us (5.4 TB/s), 700 x 650 fp32 6.7 us.  16384 x 4104 fp16 113 us (4.8 TB/s),
+// 8192 x 16384 fp16 200 us (5.4 TB/s; in fp32, where some registers spill, 5.3).  An fp32
+// stream with dz in bf16: 32768 x 8192 875 us (5.5 TB/s).
 template <int DT, int TR, int E, bool TAIL>
 __global__ __launch_bounds__(RowSum<TR>::BT) void ln_bwd_kernel(const Bwd a) {
   typedef typename DTypeTraits<DT>::raw_t raw_t;
@@ -576,16 +583,16 @@ constexpr long long LONG_ROW = 16384;     // longer rows: the kernels that loop 
 
 // Threads and elements a row (TR, E): the first that holds D.  24 elements a thread
 // stand where a class of 16 with twice the threads would be half empty and is slower
-// (us with 16 | with 24; fp16):
-//   forward    131072 x 300 52 | 47, 65536 x 650 49 | 41, 32768 x 1280 42 | 34,
-//              32768 x 2560 73 | 69, 16384 x 4104 79 | 61; but 8192 x 10240 85 | 103
-//   backward   65536 x 650 96 | 83, 32768 x 1280 84 | 73, 32768 x 2560 156 | 130, 16384 x
-//              4104 157 | 121, 8192 x 10240 159 | 142; but 131072 x 300 101 | 141
-// In fp32 they gain nothing (16384 x 5120 forward 124 | 131, backward 125 | 124) and cost
-// time where there are few rows (700 x 650: 5.8 | 7.5 and 6.7 | 9.2), so there they are
-// taken only for wide rows' gradients.
+// (us with 16 | with 24; fp16, a training step without a residual):
+//   forward    131072 x 300 57 | 44, 65536 x 650 53 | 42, 32768 x 1280 48 | 33, 16384 x
+//              4104 84 | 72 (32768 x 2560 85 | 86); but 8192 x 10240 95 | 108
+//   backward   65536 x 650 78 | 58, 32768 x 1280 71 | 52, 32768 x 2560 134 | 99, 16384 x
+//              4104 127 | 90, 8192 x 10240 195 | 108; but 131072 x 300 72 | 106
+// In fp32 they gain little (16384 x 5120 forward 143 | 147, backward 188 | 175; 65536 x 650
+// 84 | 87 and 95 | 89) and cost time where there are few rows (700 x 650: 5.7 | 7.2 and
+// 7.0 | 8.9), so there they are taken only for wide rows' gradients.
 // (The backward pass of more than 12288 elements, 16 of 1024 threads | 32 of 512: 8192 x
-// 14336 194 | 185, 4096 x 16384 fp32 274 | 217.)
+// 14336 fp16 248 | 142, 4096 x 16384 fp32 267 | 144.)
 #define LN_FWD_SIZES(F) \
   F(16, 8) F(32, 8) F(16, 24) F(64, 8) F(32, 24) F(64, 16) F(64, 24) F(128, 16) F(128, 24) \
   F(256, 16) F(256, 24) F(512, 16) F(1024, 16)
@@ -610,16 +617,21 @@ long long row_blocks(long long rows, int tr, long long cap) {
 
 // A workgroup loads the weights once for all its rows.  With 24 elements of 16 bits a
 // thread no more workgroups than run at once, three a CU (us with 4096 | 768: 5001 x
-// 4097 fp16 33 | 25, 16384 x 4104 71 | 60, 32768 x 1280 38 | 34); of 512 threads and
-// more half as many (8192 x 8191 76 | 64, with z 2048 x 8191 45 | 38), but where z and
-// s move as well and rows are many (32768 x 8192 bf16 397 | 409).
+// 4097 fp16 38 | 26, 16384 x 4104 80 | 74, 32768 x 1280 41 | 33, 65536 x 650 52 | 43).
+// Of 512 threads and more half as many.  Over 512 .. 32768 rows of 6200 .. 16384 elements
+// in 16 and 32 bits, without z: 0.78 .. 1.03 of the time (2048 x 8191 fp16 27 | 21, 8192 x
+// 8191 80 | 65, 8192 x 16384 bf16 111 | 107, 32768 x 8192 fp32 385 | 389).  With z, where s
+// moves as well, 0.82 .. 1.04 up to 4096 rows (2048 x 8191 45 | 36, 4096 x 8191 71 | 64),
+// nothing from 8192 to 16384 (0.97 .. 1.06, the last 8192 x 16384 fp32), and up to 3 %
+// lost beyond (32768 x 8192 bf16 402 | 412, 24576 x 8191 376 | 383).
 long long fwd_blocks(const Fwd& a, int tr, int e) {
   const bool half = tr >= 512 && (!a.z || a.rows < 16384);
   return row_blocks(a.rows, tr, e == 24 ? 768 : half ? 2048 : 4096);
 }
 // A workgroup leaves 8 D bytes of sums: fewer of them for longer rows (us with
-// 512 | 1024: 16384 x 4096 fp16 107 | 128, 65536 x 650 fp32 140 | 159, 8192 x 12000
-// fp16 167 | 175, 131072 x 512 fp16 117 | 104, 1048576 x 64 fp16 186 | 142).
+// 512 | 1024, the sums' kernel among them: 16384 x 4096 fp16 91 | 97, 65536 x 650 fp32
+// 99 | 110, 8192 x 12000 fp16 134 | 142; 131072 x 512 fp16 103 | 81, 131072 x 300 108 | 79,
+// 1048576 x 64 170 | 121).
 long long bwd_blocks(long long rows, long long D, int tr) {
   return row_blocks(rows, tr, D > 512 ? 512 : 1024);
 }

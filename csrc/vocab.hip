@@ -26,6 +26,9 @@
 // Both are bound by HBM: 4 to 8 instructions and one exponential an element are
 // about 60 % of the time that a 16-bit element takes to arrive.
 //
+// Times below are medians of a kernel's launches on one MI355X, three sets of inputs
+// in turn; of two sides, both with the code as it stands but for the choice.
+//
 // Defined edges: a row whose target is `ignore` is neither read nor gives a
 // gradient (0, ids -1); a row of only -inf has logprob -inf, entropy 0 and no
 // gradient; NaN or +inf in a row makes its results and its gradient NaN (a row of
@@ -47,8 +50,9 @@ constexpr int MAX_SPLITS = 64;    // workgroups a row
 constexpr long long MAX_GROUPS = 1 << 22;
 // Logits that the 256 MB of last-level cache cannot hold beside their gradient
 // are read past it (non-temporal): the backward pass would not find them there.
-// us forward + backward, streamed | not: 4096 x 131072 bf16 197 + 373 | 232 +
-// 351, 2048 x 32064 fp32 47 + 88 | 70 + 77, 700 x 10000 fp32 12 + 13 | 12 + 12.
+// us forward + backward, streamed | not: 4096 x 131072 bf16 169 + 366 | 216 + 347,
+// 8192 x 50001 bf16 146 + 285 | 177 + 276, 2048 x 32064 fp32 52 + 92 | 75 + 81, 16384 x
+// 16000 bf16 101 + 214 | 130 + 199; 700 x 10000 fp32, which it holds, 9 + 11 unstreamed.
 constexpr long long STREAM_FROM = 128LL << 20;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // An exponent far below what exp2 gives 0 for, whose product with that 0 is 0.
@@ -183,8 +187,8 @@ __device__ __forceinline__ float fold(const float* f, float c1, float& m, float&
 
 // How a workgroup walks a chunk of a row: whole 16-byte lines from the first
 // one on, element head + (j NT + thread) V in access j; the fewer than V
-// elements before that line are the last thread's.  (Accesses at odd multiples of
-// two bytes are slow: 8192 x 50001 bf16 185 us against 133 us for 50000.)
+// elements before that line are the last thread's, so that 8192 x 50001 bf16 takes as
+// long as x 50000, 143 and 145 us.  (With accesses at odd multiples of two bytes, 1.4 times.)
 template <int DT> struct Walk {
   int begin, end, n, head;        // chunk, row's length, first line's element
   template <class P> __device__ __forceinline__ Walk(P x, int b, int e, int len) {
@@ -198,9 +202,10 @@ template <int DT> struct Walk {
   }
 };
 
-// A tile is 16 elements a thread (bf16 32 | 16: 8192 x 50001 with entropy 180 |
-// 160 us, 32768 x 2000 42 | 33, 4096 x 131072 182 | 186).  Of the largest values of
-// a thread's elements SLOTS are kept, each of a run of tiles.
+// A tile is 16 elements a thread (us with 32 | 16: 8192 x 50001 bf16 139 | 132, with
+// entropy 138 | 138, with 32 alternatives too 332 | 164; 32768 x 2000 33 | 30, 4096 x
+// 131072 159 | 160).  Of the largest values of a thread's elements SLOTS are kept, each
+// of a run of tiles.
 constexpr int SLOTS = 8;
 
 template <int DT, int NT, bool ENT, bool TOP>
@@ -230,8 +235,8 @@ __device__ __forceinline__ void scan(const AS1 typename DTypeTraits<DT>::raw_t* 
 #pragma unroll
         for (int u = 0; u < U; ++u) nxt[u] = load(p + u * NT);
       }
-      // left to itself the scheduler waits for each load in some of the variants
-      // (8192 x 50001 bf16 with one alternative 177 us without both, 158 with)
+      // left to itself the scheduler moves loads to where they are used in some of the
+      // variants (8192 x 50001 bf16 with one alternative 143 us without this, 140 with)
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int u = 0; u < U; ++u) vec_to_f32<DT>(raw[u], f + u * V);
@@ -275,9 +280,9 @@ __device__ __forceinline__ void join(float c1, float* red, float& m, float& s, f
   m = s == s ? M : NAN;
 }
 
-// How many of count keys are larger than v, eight reads of LDS in flight (one by one,
-// each waited for, 32768 x 8000 bf16 with 128 alternatives takes 390 us, not 297).
-// The list goes on with zeros up to a multiple of eight.
+// How many of count keys are larger than v, eight reads of LDS in flight (us one by one,
+// each waited for | so: 32768 x 8000 bf16 with 128 alternatives 408 | 328, 65536 x 512
+// 588 | 472).  The list goes on with zeros up to a multiple of eight.
 constexpr int RANK_STEP = 8;
 __device__ __forceinline__ int larger_than(const uint64_t* list, int count, uint64_t v) {
   int n = 0;
@@ -496,8 +501,11 @@ __device__ __forceinline__ void top_of_chunk(const AS1 typename DTypeTraits<DT>:
     __syncthreads();
   }
   // Their order by counting, for each, the larger ones: quadratic, so that of many
-  // those below the k-th are dropped first (65536 x 512 bf16 with 128 of them 1871
-  // -> 888 us; with 300 candidates, 32768 x 2000, it would be 286 -> 483 us).
+  // those below the k-th are dropped first.  us never | beyond 400 | always, bf16 with
+  // 128: 65536 x 512 1320 | 476 | 477, 32768 x 1000 2064 | 246 | 243, x 2000 258 | 223 | 255,
+  // x 8000 352 | 285 | 319, 8192 x 32064 159 | 149 | 155, 16384 x 1000 fp32 126 | 113 | 159,
+  // 700 x 10000 fp32 17 | 17 | 23; with 64: 32768 x 1000 175 | 147 | 195, x 2000 181 | 151 |
+  // 157.  (Of 21 sizes one, 65536 x 512 with 64, would want fewer than 400: 577 | 551 | 395.)
   int count = sh.n;
   const uint64_t* cand = sh.cand;
   if (count > 400) {
@@ -650,12 +658,13 @@ __device__ __forceinline__ void logprob_row(const Fwd& a, long long row, float M
   }
 }
 
-// One workgroup a chunk of a row.  4096 x 131072 bf16 160 us (6.7 TB/s), 2048 x
-// 32064 fp32 with entropy 43 us (6.1 TB/s), 8192 x 50001 bf16 with entropy and 32
-// alternatives 165 us (5.0 TB/s; 131 us without either), 700 x 10000 fp32 with 5 of
-// them 12.5 us; one row of 131072 8 us, where the round trips to memory count.
-// (Six waves a SIMD also where both entropy and alternatives want registers:
-// 8192 x 50001 bf16 with 32 of them 189 -> 177 us.  Without either it costs.)
+// One workgroup a chunk of a row.  4096 x 131072 bf16 169 us (6.4 TB/s), 1792 of 2048 x
+// 32064 fp32 with entropy, in a training step, 48 us (4.7 TB/s), 8192 x 50001 bf16 with
+// entropy and 32 alternatives 186 us (4.4 TB/s; 143 us without either), 700 x 10000 fp32
+// with 5 of them 12.7 us; one row of 131072 7.4 us, where the round trips to memory count.
+// (Six waves a SIMD also where both entropy and alternatives want registers: us without
+// | with this, 8192 x 50001 bf16 with 32 of them 176 | 171, 4096 x 131072 with 20 203 | 202.
+// Elsewhere it gains nothing: 8192 x 50001 130 | 136, with entropy 137 | 140.)
 template <int DT, int NT, int MODE, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NT == 256 && ENT && TOP ? 6 : 1)))
 void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
@@ -722,7 +731,7 @@ void vocab_fwd_kernel(const Fwd a, int splits, int chunk) {
   }
 }
 
-// Joins the parts of a row (one of 131072 in 32 parts, 20 alternatives: 5.1 us, the
+// Joins the parts of a row (one of 131072 in 32 parts, 20 alternatives: 5.0 us, the
 // launch and four dependent loads).  The alternatives: every part has its own k largest
 // in order; with j of a part's keys at least as large as the r-th largest of
 // all parts' j-th keys, r j >= k, that key is a bound which at least k keys
@@ -777,7 +786,9 @@ __global__ __launch_bounds__(JOIN_NT) void vocab_join_kernel(const Fwd a, int sp
       }
       __syncthreads();
       const uint64_t bound = bound_s;
-      constexpr int U = 8;     // loads in flight (16 x 200000 bf16, 128 alternatives: 40 -> 35 us)
+      // loads in flight (us with one | eight: 16 x 200000 bf16 with 128 alternatives 26 | 20,
+      // one row of 131072 with 20 5.7 | 5.1)
+      constexpr int U = 8;
       for (int i = threadIdx.x; i < splits * a.k; i += U * NT) {
         uint64_t key[U];
 #pragma unroll
@@ -807,8 +818,8 @@ __global__ __launch_bounds__(JOIN_NT) void vocab_join_kernel(const Fwd a, int sp
 
 // One workgroup writes one tile of four 16-byte accesses a thread, then corrects
 // the few elements that carry the target's or the teacher's mass.  A read and a
-// write of every element: 4096 x 131072 bf16 355 us (6.1 TB/s; one access a thread
-// in a bare copy reaches 6.2), 2048 x 32064 fp32 84 us (5.9 TB/s).
+// write of every element: 4096 x 131072 bf16 375 us (5.7 TB/s; one access a thread
+// in a bare copy reaches 6.2), 2048 x 32064 fp32, 1792 of them read, 88 us (5.6 TB/s).
 constexpr int BWD_NT = 256;
 
 template <int DT> constexpr int bwd_chunk() { return BWD_NT * row_vec<DT>() * 4; }
@@ -884,9 +895,10 @@ __global__ __launch_bounds__(BWD_NT) void vocab_bwd_kernel(const Bwd a, int spli
 
 // Threads a workgroup.  A row of at most 8 accesses a lane is a wave's; with
 // enough rows to fill the chip by waves, one of 32 is, too, and saves the
-// workgroup's barriers (us with 64 | 256: 32768 x 8000 bf16 99 | 113, with
-// entropy 101 | 155; 16384 x 16000 with entropy 103 | 118; but 700 x 10000 fp32
-// 42 | 22).  Half of a wave's lanes have to be more than the alternatives.
+// workgroup's barriers (us with 64 | 256: 65536 x 512 bf16 33 | 116, 32768 x 2000 30 | 66,
+// 32768 x 8000 84 | 102, with entropy 88 | 125, with 32 alternatives 150 | 194; 16384 x
+// 16000 with entropy 88 | 94; but 700 x 16000 8.8 | 7.9).  Half of a wave's lanes have
+// to be more than the alternatives.
 int fwd_threads(int dt, long long rows, long long V, int k) {
   const int vec = dt == KDT_F32 ? 4 : 8;
   return k <= 32 && V <= 64 * vec * (rows >= 4096 ? 32 : 8) ? 64 : 256;

@@ -16,6 +16,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <cmath>
+
 #include "records.h"
 
 namespace {
@@ -163,7 +165,9 @@ NormGrad norm_backward_graph(const Tensor& dy, const Tensor& ds, const Tensor& s
   std::vector<int64_t> row, over;                    // the normalised dimensions, the others
   for (int64_t i = 0; i < s.dim(); ++i) (i < s.dim() - dims ? over : row).push_back(i);
   const Tensor x = s.to(at::kFloat), gy = dy.to(at::kFloat);
-  const Tensor c = x - x.mean(row, true);
+  // as csrc/ln.hip sums: scaled, so that a sum of the type's lowest values is finite
+  const double D = (double)width(s, dims), scale = std::ldexp(1.0, -1 - std::ilogb(D));
+  const Tensor c = x - (x * scale).sum(row, true) / (D * scale);
   const Tensor r = (c.square().mean(row, true) + eps).rsqrt(), h = c * r;
   const Tensor g = weight.defined() ? gy * weight.to(at::kFloat) : gy;
   NormGrad out;

@@ -39,7 +39,7 @@ struct Table {
 struct Cache {
   std::mutex mu;
   std::unordered_map<std::string, Table> map;   // its elements stay where they are
-  std::deque<Table*> pending;                   // not known to be written, in the order of their copies
+  std::deque<Table*> pending;                   // not known to be written, first copy first
   std::vector<hipEvent_t> events;               // free ones
   hipStream_t own = nullptr;
   char* dev = nullptr;      // current device arena

@@ -282,6 +282,19 @@ def plain_tensors(*tensors):
     return True
 
 
+def watched_tensors(*tensors):
+    """True for ordinary tensors under a dispatch mode or a compiler: what they are
+    to see has to be torch operations, and nothing else stands in the way."""
+    if not torch.compiler.is_compiling():
+        if not torch._C._len_torch_dispatch_stack() or torch._C._is_tracing() \
+                or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0:
+            return False
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return True
+
+
 def stream(device=None):
     return c_vp(torch.cuda.current_stream(device).cuda_stream)
 

@@ -12,7 +12,9 @@ Logits are (..., V) of fp32, bf16 or fp16 (fp64 too on the CPU), any strides;
 everything is computed and returned in fp32 (fp64 for fp64), the gradient in
 the logits' type.  GPU tensors run on the HIP kernels (hipGraph-capturable,
 bitwise reproducible, no host synchronisation; the autograd nodes are C++,
-csrc/torch_ops.cpp), CPU tensors on the same formulas in torch.  Neither op has a second derivative.
+csrc/torch_ops.cpp), CPU tensors on the same formulas in torch; so does a call under
+a dispatch mode (a FLOP counter, selective checkpointing) or a compiler, which have
+to see operations.  Neither op has a second derivative.
 
 What a kernel meets on the device cannot raise without a synchronisation: a
 target out of range makes its row's log probability and that one's gradient NaN,
@@ -74,13 +76,17 @@ def _check_ids(name, what, t, shape, device):
             name, what, t.device, device))
 
 
-def _check_plain(name, *tensors):
-    if not _lib.plain_tensors(*tensors):
+def _native(name, *tensors):
+    """Whether the kernels run: the formulas below do elsewhere."""
+    if _lib.plain_tensors(*tensors):
+        return _lib.use_native(tensors[0])
+    if not _lib.watched_tensors(*tensors):
         raise TypeError('{}: takes ordinary tensors, outside functorch transforms, forward-mode '
-                        'levels, dispatch modes and traces'.format(name))
+                        'levels and traces'.format(name))
+    return False
 
 
-# -------------------------------------------------------- CPU: the formulas
+# ------------------------------------------------ CPU tensors, modes: the formulas
 def _cpu_stats(x, inv_t):
     """(x as computed in, M, L, lp): csrc/vocab.hip's names."""
     x = x if x.dtype == torch.float64 else x.float()
@@ -110,7 +116,7 @@ class _TokenLogprobs(torch.autograd.Function):
         shape = logits.shape[:-1]
         rows = logits.reshape(-1, logits.shape[-1])
         x, M, _, lp = _cpu_stats(rows, inv_t)
-        skip = torch.zeros(len(x), dtype=torch.bool) if targets is None else \
+        skip = torch.zeros(len(x), dtype=torch.bool, device=x.device) if targets is None else \
             targets.reshape(-1) == ignore
         ctx.inv_t, ctx.skip = inv_t, skip
         ctx.set_materialize_grads(False)
@@ -121,8 +127,10 @@ class _TokenLogprobs(torch.autograd.Function):
         if entropy:
             h = torch.where(skip, 0.0, _cpu_entropy(lp, M == -math.inf)).view(shape)
         if k:
-            # stable, so that equal values keep the order of their indices
-            ids = torch.sort(x, dim=1, descending=True, stable=True)[1][:, :k]
+            # stable, so that equal values keep the order of their indices; a device's sort
+            # may tell zeros and NaN apart by their signs
+            key = torch.where(torch.isnan(x), math.nan, x + 0.0)
+            ids = torch.sort(key, dim=1, descending=True, stable=True)[1][:, :k]
             ti = ids.masked_fill(skip[:, None], -1).view(shape + (k,))
             tl = lp.gather(1, ids).masked_fill(skip[:, None], -math.inf).view(shape + (k,))
             ctx.mark_non_differentiable(tl, ti)
@@ -181,9 +189,8 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=False, temperature=1.0
             min(TOP_MAX, logits.shape[-1]), top_k))
     if targets is None and not k and not entropy:
         raise ValueError('token_logprobs: nothing asked for (no targets, top_k 0, no entropy)')
-    _check_plain('token_logprobs', logits, targets)
-    call = _lib.torch_ops().token_logprobs.default if _lib.use_native(logits) else \
-        _TokenLogprobs.apply
+    call = _lib.torch_ops().token_logprobs.default if _native('token_logprobs', logits, targets) \
+        else _TokenLogprobs.apply
     return TokenLogprobs(*call(logits, targets, k, bool(entropy), inv_t, int(ignore_index)))
 
 
@@ -270,7 +277,6 @@ def topk_distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0):
         raise ValueError('{}: the teacher is a constant; detach teacher_logits'.format(name))
     if logits.is_cuda and teacher_logits.dtype == torch.float64:
         teacher_logits = teacher_logits.float()
-    _check_plain(name, logits, teacher_ids, teacher_logits)
-    if _lib.use_native(logits):
+    if _native(name, logits, teacher_ids, teacher_logits):
         return _lib.torch_ops().topk_distill.default(logits, teacher_ids, teacher_logits, inv_t)
     return _TopkDistill.apply(logits, teacher_ids.to(torch.int64), teacher_logits, inv_t)
